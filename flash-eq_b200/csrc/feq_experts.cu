@@ -1,0 +1,636 @@
+// feq_experts.cu -- tokens to experts and back: the routing decision, the stable sort of the
+// chosen (token, choice) pairs by expert, the rows' move to sorted order and the weighted sum back,
+// and the gradients.
+//
+//   route     ids[n, :] = the top_k largest logits of token n, downwards (equal logits: the lower
+//             expert first; -inf is never chosen: id -1, weight 0); weights = softmax over the chosen
+//             logits, or the chosen entries of the softmax over all of them.  slots[n, j] = the
+//             place of pair n * k + j in the stable order by expert, pairs without an expert last;
+//             offsets[e] = the first place of expert e.
+//   dispatch  sorted[slots[n, j]] = x[n]; rows without an expert are 0
+//   combine   out[n] = sum_j w[n, j] y[slots[n, j]] over the pairs that have an expert
+//   backward  grad_x[n] = sum_j grad_sorted[slots[n, j]] (a combine with weights of 1);
+//             grad_y[slots[n, j]] = w[n, j] grad_out[n], grad_w[n, j] = <grad_out[n], y[slots[n, j]]>;
+//             grad_logits from grad_w through the softmax
+//
+// slots is a permutation of the n * k places, so every kernel walks tokens in order, reads or
+// writes the token's row once, and needs no atomics: results do not depend on the launch.  All
+// of them are bound by HBM (the rows), the small ones by launches: up to kSmallPairs pairs the whole
+// routing is one block, beyond that three launches (choose and count per block, prefix per
+// expert over the blocks, place).
+#include "feq_token.cuh"
+
+namespace feq {
+namespace experts {
+
+using namespace token;
+
+constexpr int kMaxExperts = 512, kMaxTopK = 32;
+constexpr int kPerLane = kMaxExperts / 32;
+constexpr int kSmallPairs = 4096;             // one block routes these
+constexpr int kSmallThreads = 1024;
+constexpr int kPlaceThreads = 256;
+constexpr int kPlacePairs = 2048;             // pairs of one placing block
+
+struct Route {
+    const void *logits;
+    int64_t tokens, stride;
+    int experts, top_k, normalize;
+    int32_t *ids;                             // (tokens, k), -1 where a pair has no expert
+    float *weights;                           // (tokens, k)
+    int32_t *slots, *offsets;                 // (tokens, k), (experts + 1)
+    int32_t *counts;                          // (experts + 1, blocks)
+    int blocks, tokens_per_block;
+};
+
+// Order-preserving image of a float, 0 for -inf (never chosen) and the largest for NaN.
+__device__ __forceinline__ uint32_t rank_key(float v) {
+    if (v != v) return 0xffffffffu;
+    if (v == -INFINITY) return 0u;
+    const uint32_t u = __float_as_uint(v + 0.0f);      // -0 equals +0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One warp chooses the experts of one token; lane j < top_k ends up with choice j (id -1: none).
+template <typename T>
+__device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, float &my_w) {
+    const int lane = threadIdx.x & 31;
+    const T *row = static_cast<const T *>(a.logits) + n * a.stride;
+    float v[kPerLane];
+    uint32_t key[kPerLane];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; i++) {
+        const int e = i * 32 + lane;
+        if (i * 32 >= a.experts) break;
+        v[i] = e < a.experts ? to_f32(row[e]) : -INFINITY;
+        key[i] = rank_key(v[i]);
+        top = max(top, key[i]);
+    }
+    my_id = -1;
+    float my_v = -INFINITY, biggest = 0.0f;
+    for (int j = 0; j < a.top_k; j++) {
+        const uint32_t best = __reduce_max_sync(0xffffffffu, top);
+        if (best == 0u) break;                          // nothing but -inf is left
+        int e = 0x7fffffff;
+        float val = 0.0f;
+#pragma unroll
+        for (int i = kPerLane - 1; i >= 0; i--) {
+            if (i * 32 >= a.experts) continue;
+            if (key[i] == best) {
+                e = i * 32 + lane;
+                val = v[i];
+            }
+        }
+        const int win = __reduce_min_sync(0xffffffffu, e);
+        val = __shfl_sync(0xffffffffu, val, win & 31);
+        if (j == 0) biggest = val;
+        if (lane == j) {
+            my_id = win;
+            my_v = val;
+        }
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < kPerLane; i++) {
+            if (i * 32 >= a.experts) break;
+            if (i * 32 + lane == win) key[i] = 0u;
+            top = max(top, key[i]);
+        }
+    }
+    float total;
+    my_w = my_id >= 0 ? expf(my_v - biggest) : 0.0f;
+    if (a.normalize) {
+        total = lane_sum(my_w, 32);
+    } else {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPerLane; i++) {
+            if (i * 32 >= a.experts) break;
+            s += expf(v[i] - biggest);
+        }
+        total = lane_sum(s, 32);
+    }
+    if (my_id >= 0) my_w /= total;
+}
+
+// Counts of the pairs [lo, hi) of `key` (experts for none) per expert, one warp, into hist.
+__device__ __forceinline__ void warp_count(const int16_t *key, int lo, int hi, int32_t *hist) {
+    const int lane = threadIdx.x & 31;
+    for (int p0 = lo; p0 < hi; p0 += 32) {
+        const int p = p0 + lane;
+        const int k = p < hi ? key[p] : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, k);
+        if (k >= 0 && lane == __ffs(same) - 1) hist[k] += __popc(same);
+        __syncwarp();
+    }
+}
+
+// Places of the pairs [lo, hi) in order, next free place per expert in hist (advanced).
+__device__ __forceinline__ void warp_place(const int16_t *key, int lo, int hi, int32_t *hist, int32_t *slots) {
+    const int lane = threadIdx.x & 31;
+    for (int p0 = lo; p0 < hi; p0 += 32) {
+        const int p = p0 + lane;
+        const int k = p < hi ? key[p] : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, k);
+        if (k >= 0) slots[p] = hist[k] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (k >= 0 && lane == __ffs(same) - 1) hist[k] += __popc(same);
+        __syncwarp();
+    }
+}
+
+// Exclusive prefix of count[0 .. n) in place by one block; count[n] = the total.  n <= 2 * blockDim.
+__device__ __forceinline__ void block_prefix(int32_t *count, int n, int32_t *scratch) {
+    // (n is at most 513: one warp walks it 32 at a time)
+    if (threadIdx.x < 32) {
+        int32_t base = 0;
+        for (int i0 = 0; i0 < n; i0 += 32) {
+            const int i = i0 + threadIdx.x;
+            const int32_t c = i < n ? count[i] : 0;
+            int32_t s = c;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+                if ((int)threadIdx.x >= o) s += u;
+            }
+            if (i < n) scratch[i] = base + s - c;
+            base += __shfl_sync(0xffffffffu, s, 31);
+        }
+    }
+    __syncthreads();
+}
+
+// Warps' counts hist (warps, stride) -> first places: starts[k] + the counts of the warps before.
+__device__ __forceinline__ void warp_starts(int32_t *hist, int warps, int n, int stride, const int32_t *starts) {
+    for (int k = threadIdx.x; k < n; k += blockDim.x) {
+        int32_t at = starts[k];
+        for (int w = 0; w < warps; w++) {
+            const int32_t c = hist[w * stride + k];
+            hist[w * stride + k] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+}
+
+// The whole routing of up to kSmallPairs pairs in one block.
+template <typename T>
+__global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const Route a) {
+    extern __shared__ int32_t sh[];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nk = a.experts + 1, pairs = (int)a.tokens * a.top_k;
+    int32_t *hist = sh, *count = hist + warps * nk, *starts = count + nk;
+    int16_t *key = reinterpret_cast<int16_t *>(starts + nk);
+    for (int i = threadIdx.x; i < warps * nk; i += blockDim.x) hist[i] = 0;
+    for (int n = warp; n < (int)a.tokens; n += warps) {
+        int id;
+        float w;
+        choose<T>(a, n, id, w);
+        if (lane < a.top_k) {
+            const int p = n * a.top_k + lane;
+            a.ids[p] = id;
+            a.weights[p] = w;
+            key[p] = (int16_t)(id < 0 ? a.experts : id);
+        }
+    }
+    __syncthreads();
+    const int per = ((pairs + warps - 1) / warps + 31) & ~31;
+    const int lo = min(warp * per, pairs), hi = min(lo + per, pairs);
+    warp_count(key, lo, hi, hist + warp * nk);
+    __syncthreads();
+    for (int k = threadIdx.x; k < nk; k += blockDim.x) {
+        int32_t c = 0;
+        for (int w = 0; w < warps; w++) c += hist[w * nk + k];
+        count[k] = c;
+    }
+    __syncthreads();
+    block_prefix(count, nk, starts);
+    for (int k = threadIdx.x; k < nk; k += blockDim.x) a.offsets[k] = starts[k];
+    warp_starts(hist, warps, nk, nk, starts);
+    warp_place(key, lo, hi, hist + warp * nk, a.slots);
+}
+
+// Step 1 of 3: choose, and count a block's pairs per expert.
+template <typename T>
+__global__ void __launch_bounds__(kPlaceThreads) route_choose_kernel(const Route a) {
+    extern __shared__ int32_t sh[];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int nk = a.experts + 1;
+    for (int i = threadIdx.x; i < nk; i += blockDim.x) sh[i] = 0;
+    __syncthreads();
+    const int64_t n0 = (int64_t)blockIdx.x * a.tokens_per_block, n1 = min64(n0 + a.tokens_per_block, a.tokens);
+    for (int64_t n = n0 + warp; n < n1; n += warps) {
+        int id;
+        float w;
+        choose<T>(a, n, id, w);
+        if (lane < a.top_k) {
+            const int64_t p = n * a.top_k + lane;
+            a.ids[p] = id;
+            a.weights[p] = w;
+            atomicAdd(&sh[id < 0 ? a.experts : id], 1);      // integers: any order gives the same counts
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nk; i += blockDim.x) a.counts[(int64_t)i * a.blocks + blockIdx.x] = sh[i];
+}
+
+// Step 2 of 3: one block per expert, exclusive prefix over the placing blocks; the expert's total
+// goes to offsets[expert] until step 3 turns the totals into first places.
+__global__ void __launch_bounds__(256) route_prefix_kernel(const Route a, int32_t *totals) {
+    __shared__ int32_t part[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int32_t *c = a.counts + (int64_t)blockIdx.x * a.blocks;
+    int32_t base = 0;
+    for (int i0 = 0; i0 < a.blocks; i0 += 256) {
+        const int i = i0 + threadIdx.x;
+        const int32_t v = i < a.blocks ? c[i] : 0;
+        int32_t s = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane == 31) part[warp] = s;
+        __syncthreads();
+        int32_t before = 0, all = 0;
+        for (int w = 0; w < 8; w++) {
+            if (w < warp) before += part[w];
+            all += part[w];
+        }
+        if (i < a.blocks) c[i] = base + before + s - v;
+        base += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) totals[blockIdx.x] = base;
+}
+
+// Step 3 of 3: the pairs' places.
+__global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(const Route a, const int32_t *totals) {
+    extern __shared__ int32_t sh[];
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+    const int nk = a.experts + 1;
+    int32_t *hist = sh, *count = hist + warps * nk, *starts = count + nk;
+    int16_t *key = reinterpret_cast<int16_t *>(starts + nk);
+    const int64_t p0 = (int64_t)blockIdx.x * a.tokens_per_block * a.top_k;
+    const int pairs = (int)min64((int64_t)a.tokens_per_block * a.top_k, a.tokens * a.top_k - p0);
+    for (int i = threadIdx.x; i < warps * nk; i += blockDim.x) hist[i] = 0;
+    for (int i = threadIdx.x; i < nk; i += blockDim.x) count[i] = totals[i];
+    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
+        const int id = a.ids[p0 + p];
+        key[p] = (int16_t)(id < 0 ? a.experts : id);
+    }
+    __syncthreads();
+    block_prefix(count, nk, starts);
+    if (blockIdx.x == 0)
+        for (int k = threadIdx.x; k < nk; k += blockDim.x) a.offsets[k] = starts[k];
+    __syncthreads();
+    for (int k = threadIdx.x; k < nk; k += blockDim.x) starts[k] += a.counts[(int64_t)k * a.blocks + blockIdx.x];
+    const int per = ((pairs + warps - 1) / warps + 31) & ~31;
+    const int lo = min(warp * per, pairs), hi = min(lo + per, pairs);
+    warp_count(key, lo, hi, hist + warp * nk);
+    __syncthreads();
+    warp_starts(hist, warps, nk, nk, starts);
+    warp_place(key, lo, hi, hist + warp * nk, a.slots + p0);
+}
+
+// grad_logits of the weights; one warp per token.
+template <typename T>
+__global__ void __launch_bounds__(256)
+route_bwd_kernel(const T *__restrict__ logits, int64_t stride, int64_t tokens, int E, int k, int normalize,
+                 const int32_t *__restrict__ ids, const float *__restrict__ w, const float *__restrict__ gw,
+                 T *__restrict__ out) {
+    const int lane = threadIdx.x & 31;
+    const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (n >= tokens) return;
+    const int id = lane < k ? ids[n * k + lane] : -1;
+    const float wj = id >= 0 ? w[n * k + lane] : 0.0f, g = id >= 0 ? gw[n * k + lane] : 0.0f;
+    const float share = lane_sum(wj * g, 32);
+    float biggest = 0.0f, total = 1.0f;
+    if (!normalize) {
+        const int first = __shfl_sync(0xffffffffu, id, 0);
+        if (first >= 0 && first < E) {
+            biggest = to_f32(logits[n * stride + first]);
+            float s = 0.0f;
+            for (int e = lane; e < E; e += 32) s += expf(to_f32(logits[n * stride + e]) - biggest);
+            total = lane_sum(s, 32);
+        }
+    }
+    for (int e0 = 0; e0 < E; e0 += 32) {
+        const int e = e0 + lane;
+        float v = 0.0f, spread = 0.0f;
+        for (int j = 0; j < k; j++) {
+            const int ej = __shfl_sync(0xffffffffu, id, j);
+            const float a = __shfl_sync(0xffffffffu, wj, j), b = __shfl_sync(0xffffffffu, g, j);
+            if (ej == e) {
+                v = a * b;
+                spread = a;
+            }
+        }
+        if (e < E) {
+            if (!normalize) spread = expf(to_f32(logits[n * stride + e]) - biggest) / total;
+            out[n * E + e] = from_f32<T>(v - spread * share);
+        }
+    }
+}
+
+// ---- rows ------------------------------------------------------------------------------------
+struct Rows {
+    const void *a, *b;                        // read: token rows (a), sorted rows (b)
+    void *out;
+    int64_t tokens, a_stride, b_stride;
+    int top_k, experts;
+    int64_t width;                            // elements of a row
+    const int32_t *slots, *offsets;
+    const float *w;
+    float *gw;
+};
+
+// A pair's place: its slot where it has an expert, -1 where it has none; a slot outside the sorted
+// rows (not from expert_route) counts as `outside` and is not touched.
+enum : int { kNoExpert = -1, kOutside = -2 };
+__device__ __forceinline__ int place_of(const Rows &a, int64_t pair, int kept) {
+    const int slot = a.slots[pair];
+    if (slot < 0 || slot >= a.tokens * a.top_k) return kOutside;
+    return slot < kept ? slot : kNoExpert;
+}
+
+// The token's row goes to its top_k places (x[n] -> sorted); pairs without an expert get zeros.
+// A unit is `V` elements of one token: units of a row lie side by side.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) dispatch_kernel(const Rows a) {
+    const int64_t units = a.width / V, total = a.tokens * units;
+    const int kept = a.offsets[a.experts];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i / units, c = (i - n * units) * V;
+        const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.a) + n * a.a_stride + c);
+        Pack<T, V> z;
+#pragma unroll
+        for (int q = 0; q < V; q++) z.v[q] = from_f32<T>(0.0f);
+        for (int j = 0; j < a.top_k; j++) {
+            const int64_t slot = a.slots[n * a.top_k + j];
+            const int at = place_of(a, n * a.top_k + j, kept);
+            if (at == kOutside) continue;
+            *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + slot * a.width + c) = at >= 0 ? v : z;
+        }
+    }
+}
+
+// out[n] = sum_j w[n, j] sorted[slots[n, j]] (w null: 1), summed in float32 in the order of j.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_kernel(const Rows a) {
+    const int64_t units = a.width / V, total = a.tokens * units;
+    const int kept = a.offsets[a.experts];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i / units, c = (i - n * units) * V;
+        float s[V];
+#pragma unroll
+        for (int q = 0; q < V; q++) s[q] = 0.0f;
+        for (int j = 0; j < a.top_k; j++) {
+            const int64_t p = n * a.top_k + j;
+            const int64_t slot = place_of(a, p, kept);
+            if (slot < 0) continue;
+            const Pack<T, V> v =
+                *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.b) + slot * a.b_stride + c);
+            const float w = a.w ? a.w[p] : 1.0f;
+#pragma unroll
+            for (int q = 0; q < V; q++) s[q] += w * to_f32(v.v[q]);
+        }
+        Pack<T, V> o;
+#pragma unroll
+        for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(s[q]);
+        *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + n * a.width + c) = o;
+    }
+}
+
+// grad_y[slot] = w grad_out[n] and grad_w = <grad_out[n], y[slot]>: one warp per token.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) combine_bwd_kernel(const Rows a) {
+    const int lane = threadIdx.x & 31;
+    const int kept = a.offsets[a.experts];
+    for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < a.tokens; n += (int64_t)gridDim.x * 8) {
+        const T *g = static_cast<const T *>(a.a) + n * a.a_stride;
+        for (int j = 0; j < a.top_k; j++) {
+            const int64_t p = n * a.top_k + j;
+            const int64_t slot = a.slots[p];
+            const int at = place_of(a, p, kept);
+            if (at == kOutside) {
+                if (lane == 0) a.gw[p] = 0.0f;
+                continue;
+            }
+            const bool live = at >= 0;
+            const T *y = static_cast<const T *>(a.b) + slot * a.b_stride;
+            T *out = static_cast<T *>(a.out) + slot * a.width;
+            const float w = a.w[p];
+            float dot = 0.0f;
+            for (int64_t c = lane * V; c < a.width; c += 32 * V) {
+                Pack<T, V> o;
+#pragma unroll
+                for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(0.0f);
+                if (live) {
+                    const Pack<T, V> u = *reinterpret_cast<const Pack<T, V> *>(g + c);
+                    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(y + c);
+#pragma unroll
+                    for (int q = 0; q < V; q++) {
+                        const float f = to_f32(u.v[q]);
+                        dot += f * to_f32(v.v[q]);
+                        o.v[q] = from_f32<T>(w * f);
+                    }
+                }
+                *reinterpret_cast<Pack<T, V> *>(out + c) = o;
+            }
+            dot = lane_sum(dot, 32);
+            if (lane == 0) a.gw[p] = dot;
+        }
+    }
+}
+
+int route_plan(int64_t tokens, int top_k, int *per) {
+    const int t = kPlacePairs / top_k;
+    *per = t;
+    return (int)((tokens + t - 1) / t);
+}
+
+int check(int64_t tokens, int top_k, int experts) {
+    if (tokens < 0 || top_k < 1 || experts < 1 || top_k > experts) return FEQ_ERR_INVALID_ARGUMENT;
+    if (experts > kMaxExperts || top_k > kMaxTopK || tokens * top_k >= (int64_t)1 << 31) return FEQ_ERR_UNSUPPORTED;
+    return FEQ_OK;
+}
+
+unsigned row_grid(int64_t units) { return (unsigned)max64(1, min64((units + 255) / 256, (int64_t)sm_count() * 16)); }
+
+}  // namespace experts
+}  // namespace feq
+
+using namespace feq;
+using namespace feq::token;
+
+extern "C" size_t feq_expert_route_workspace_bytes(int64_t tokens, int32_t top_k, int32_t experts) {
+    if (experts::check(tokens, top_k, experts) != FEQ_OK) return 0;
+    int per;
+    const int blocks = experts::route_plan(tokens, top_k, &per);
+    return (size_t)(experts + 1) * ((size_t)blocks + 1) * sizeof(int32_t);
+}
+
+extern "C" int feq_expert_route(const void *logits, int64_t tokens, int64_t stride, int32_t num_experts, int32_t top_k,
+                                int32_t dtype, int32_t normalize, int32_t *ids, float *weights, int32_t *slots,
+                                int32_t *offsets, void *workspace, size_t workspace_bytes, feq_stream_t stream) {
+    const int rc = experts::check(tokens, top_k, num_experts);
+    if (rc != FEQ_OK) return rc;
+    if (!dtype_ok(dtype) || stride < 0 || !offsets) return FEQ_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (tokens == 0) {
+        FEQ_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(num_experts + 1) * sizeof(int32_t), s));
+        return FEQ_OK;
+    }
+    if (!logits || !ids || !weights || !slots) return FEQ_ERR_INVALID_ARGUMENT;
+    ProfScope prof("expert_route", s);
+    experts::Route a = {};
+    a.logits = logits;
+    a.tokens = tokens;
+    a.stride = stride;
+    a.experts = num_experts;
+    a.top_k = top_k;
+    a.normalize = normalize;
+    a.ids = ids;
+    a.weights = weights;
+    a.slots = slots;
+    a.offsets = offsets;
+    const int nk = num_experts + 1;
+    if (tokens * top_k <= experts::kSmallPairs) {
+        const int warps = (int)min64(experts::kSmallThreads / 32, max64(tokens, 1));
+        const size_t smem = (size_t)(warps + 2) * nk * 4 + (size_t)tokens * top_k * 2;
+        FEQ_TOKEN_TYPE(dtype, {
+            auto kern = experts::route_small_kernel<T>;
+            if (smem > 48 * 1024)
+                FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            kern<<<1, warps * 32, smem, s>>>(a);
+        })
+        FEQ_LAUNCH_CHECK();
+        return FEQ_OK;
+    }
+    if (!workspace || workspace_bytes < feq_expert_route_workspace_bytes(tokens, top_k, num_experts))
+        return FEQ_ERR_WORKSPACE;
+    a.blocks = experts::route_plan(tokens, top_k, &a.tokens_per_block);
+    a.counts = static_cast<int32_t *>(workspace);
+    int32_t *totals = a.counts + (size_t)nk * a.blocks;
+    const size_t smem = (size_t)(experts::kPlaceThreads / 32 + 2) * nk * 4 + experts::kPlacePairs * 2;
+    FEQ_TOKEN_TYPE(dtype, experts::route_choose_kernel<T><<<a.blocks, experts::kPlaceThreads, nk * 4, s>>>(a);)
+    FEQ_LAUNCH_CHECK();
+    experts::route_prefix_kernel<<<nk, 256, 0, s>>>(a, totals);
+    FEQ_LAUNCH_CHECK();
+    experts::route_place_kernel<<<a.blocks, experts::kPlaceThreads, smem, s>>>(a, totals);
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}
+
+extern "C" int feq_expert_route_bwd(const void *logits, int64_t tokens, int64_t stride, int32_t num_experts,
+                                    int32_t top_k, int32_t dtype, int32_t normalize, const int32_t *ids,
+                                    const float *weights, const float *grad_weights, void *grad_logits,
+                                    feq_stream_t stream) {
+    const int rc = experts::check(tokens, top_k, num_experts);
+    if (rc != FEQ_OK) return rc;
+    if (!dtype_ok(dtype) || stride < 0) return FEQ_ERR_INVALID_ARGUMENT;
+    if (tokens == 0) return FEQ_OK;
+    if (!logits || !ids || !weights || !grad_weights || !grad_logits) return FEQ_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    ProfScope prof("expert_route_bwd", s);
+    const unsigned grid = (unsigned)((tokens + 7) / 8);
+    FEQ_TOKEN_TYPE(dtype, experts::route_bwd_kernel<T><<<grid, 256, 0, s>>>(
+                              static_cast<const T *>(logits), stride, tokens, num_experts, top_k, normalize, ids,
+                              weights, grad_weights, static_cast<T *>(grad_logits));)
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}
+
+namespace feq {
+namespace experts {
+static int rows_args(Rows *r, int64_t tokens, int32_t top_k, int32_t num_experts, int64_t width, int32_t dtype,
+                     const int32_t *slots, const int32_t *offsets) {
+    const int rc = check(tokens, top_k, num_experts);
+    if (rc != FEQ_OK) return rc;
+    if (width < 1 || !dtype_ok(dtype) || !offsets || (tokens && !slots)) return FEQ_ERR_INVALID_ARGUMENT;
+    r->tokens = tokens;
+    r->top_k = top_k;
+    r->experts = num_experts;
+    r->width = width;
+    r->slots = slots;
+    r->offsets = offsets;
+    return FEQ_OK;
+}
+}  // namespace experts
+}  // namespace feq
+
+extern "C" int feq_expert_dispatch(const void *x, int64_t tokens, int64_t x_stride, int64_t width, int32_t dtype,
+                                   int32_t top_k, int32_t num_experts, const int32_t *slots, const int32_t *offsets,
+                                   void *sorted, feq_stream_t stream) {
+    experts::Rows r = {};
+    const int rc = experts::rows_args(&r, tokens, top_k, num_experts, width, dtype, slots, offsets);
+    if (rc != FEQ_OK) return rc;
+    if (x_stride < 0) return FEQ_ERR_INVALID_ARGUMENT;
+    if (tokens == 0) return FEQ_OK;
+    if (!x || !sorted) return FEQ_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    ProfScope prof("expert_dispatch", s);
+    r.a = x;
+    r.a_stride = x_stride;
+    r.out = sorted;
+    const size_t es = dtype_bytes(dtype);
+    const int vec = vector_elems((uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)sorted | (uint64_t)x_stride * es |
+                                     (uint64_t)width * es, es);
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::dispatch_kernel<T, V><<<experts::row_grid(tokens * (width / V)),
+                                                                             256, 0, s>>>(r);))
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}
+
+extern "C" int feq_expert_combine(const void *sorted, int64_t sorted_stride, int64_t tokens, int64_t width,
+                                  int32_t dtype, int32_t top_k, int32_t num_experts, const int32_t *slots,
+                                  const int32_t *offsets, const float *weights, void *out, feq_stream_t stream) {
+    experts::Rows r = {};
+    const int rc = experts::rows_args(&r, tokens, top_k, num_experts, width, dtype, slots, offsets);
+    if (rc != FEQ_OK) return rc;
+    if (sorted_stride < 0) return FEQ_ERR_INVALID_ARGUMENT;
+    if (tokens == 0) return FEQ_OK;
+    if (!sorted || !out) return FEQ_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    ProfScope prof("expert_combine", s);
+    r.b = sorted;
+    r.b_stride = sorted_stride;
+    r.out = out;
+    r.w = weights;
+    const size_t es = dtype_bytes(dtype);
+    const int vec = vector_elems((uint64_t)(uintptr_t)sorted | (uint64_t)(uintptr_t)out |
+                                     (uint64_t)sorted_stride * es | (uint64_t)width * es, es);
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::combine_kernel<T, V><<<experts::row_grid(tokens * (width / V)),
+                                                                            256, 0, s>>>(r);))
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}
+
+extern "C" int feq_expert_combine_bwd(const void *grad_out, int64_t grad_stride, const void *sorted,
+                                      int64_t sorted_stride, int64_t tokens, int64_t width, int32_t dtype,
+                                      int32_t top_k, int32_t num_experts, const int32_t *slots, const int32_t *offsets,
+                                      const float *weights, void *grad_sorted, float *grad_weights,
+                                      feq_stream_t stream) {
+    experts::Rows r = {};
+    const int rc = experts::rows_args(&r, tokens, top_k, num_experts, width, dtype, slots, offsets);
+    if (rc != FEQ_OK) return rc;
+    if (grad_stride < 0 || sorted_stride < 0) return FEQ_ERR_INVALID_ARGUMENT;
+    if (tokens == 0) return FEQ_OK;
+    if (!grad_out || !sorted || !weights || !grad_sorted || !grad_weights) return FEQ_ERR_INVALID_ARGUMENT;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    ProfScope prof("expert_combine_bwd", s);
+    r.a = grad_out;
+    r.a_stride = grad_stride;
+    r.b = sorted;
+    r.b_stride = sorted_stride;
+    r.out = grad_sorted;
+    r.w = weights;
+    r.gw = grad_weights;
+    const size_t es = dtype_bytes(dtype);
+    const int vec = vector_elems((uint64_t)(uintptr_t)grad_out | (uint64_t)(uintptr_t)sorted |
+                                     (uint64_t)(uintptr_t)grad_sorted | (uint64_t)grad_stride * es |
+                                     (uint64_t)sorted_stride * es | (uint64_t)width * es, es);
+    const unsigned grid = (unsigned)min64((tokens + 7) / 8, (int64_t)sm_count() * 32);
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::combine_bwd_kernel<T, V><<<grid, 256, 0, s>>>(r);))
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}

@@ -5,17 +5,27 @@ the per-edge work (Wigner-D basis, edgewise linear, attention softmax, pooling)
 runs in hand-written sm_100a kernels (libflasheq_b200.so) called through a C ABI.
 """
 from .cuda import CUDANotAvailableError
+from .cuda.token_autograd import (
+    ExpertRoute,
+    expert_combine,
+    expert_dispatch,
+    expert_linear,
+    expert_route,
+    layer_norm,
+)
 from .graph import Graph
 from .layers import (
     EquivariantAttention,
     EquivariantEdgeAttention,
     EquivariantEdgewiseLinear,
+    EquivariantExperts,
     EquivariantGating,
     EquivariantLayerNorm,
     EquivariantLinear,
     EquivariantTransformer,
     EquivariantTransformerBlock,
     GraphPooling,
+    InvariantLayerNorm,
     RepNorm,
     S2Activation,
     SeparableEquivariantLayerNorm,
@@ -35,5 +45,6 @@ __all__ = [
     "EquivariantLayerNorm", "SeparableEquivariantLayerNorm", "GraphPooling", "EquivariantEdgeAttention",
     "S2Activation", "SeparableS2Activation", "EquivariantTransformerBlock", "EquivariantTransformer",
     "WignerDBasis", "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet", "SequencePositionEncoding",
+    "EquivariantExperts", "InvariantLayerNorm", "layer_norm", "ExpertRoute", "expert_route", "expert_dispatch", "expert_linear", "expert_combine",
     "S2Grid", "real_spherical_harmonics", "lebedev_grid", "CUDANotAvailableError", "patch",
 ]

@@ -67,7 +67,18 @@ class FeqAttnBwdArgs(ctypes.Structure):
     ]
 
 
-FEQ_ABI_VERSION = 4   # must equal feq_abi_version() of the loaded library
+class FeqExpertLinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("x_row_stride", ctypes.c_int64), ("x_comp_stride", ctypes.c_int64), ("weight", c_vp),
+        ("bias", c_vp), ("offsets", c_vp), ("rows", ctypes.c_int64), ("lvals", c_i32p), ("n_lvals", ctypes.c_int32),
+        ("num_experts", ctypes.c_int32), ("c_in", ctypes.c_int32), ("c_out", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("out", c_vp), ("grad_out", c_vp), ("grad_row_stride", ctypes.c_int64),
+        ("grad_comp_stride", ctypes.c_int64), ("grad_x", c_vp), ("grad_weight", c_vp), ("grad_bias", c_vp),
+        ("status", c_vp),
+    ]
+
+
+FEQ_ABI_VERSION = 5   # must equal feq_abi_version() of the loaded library
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -164,6 +175,28 @@ SIGNATURES = {
     "feq_segment_pool_bwd": (ctypes.c_int, [c_vp, ctypes.c_int64, c_vp, ctypes.c_int32, c_vp, c_vp, c_vp,
                                             ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp,
                                             c_vp, c_vp, c_vp]),
+    "feq_layer_norm_fwd": (ctypes.c_int, [c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, c_vp,
+                                          c_vp, ctypes.c_int32, ctypes.c_float, c_vp, c_vp, c_vp, c_vp]),
+    "feq_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32]),
+    "feq_layer_norm_bwd": (ctypes.c_int, [c_vp, ctypes.c_int64, c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                          ctypes.c_int32, c_vp, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                          ctypes.c_size_t, c_vp]),
+    "feq_expert_route_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]),
+    "feq_expert_route": (ctypes.c_int, [c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                        ctypes.c_int32, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp, c_vp, ctypes.c_size_t,
+                                        c_vp]),
+    "feq_expert_route_bwd": (ctypes.c_int, [c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                            ctypes.c_int32, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "feq_expert_dispatch": (ctypes.c_int, [c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                           ctypes.c_int32, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp]),
+    "feq_expert_combine": (ctypes.c_int, [c_vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32,
+                                          ctypes.c_int32, ctypes.c_int32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "feq_expert_combine_bwd": (ctypes.c_int, [c_vp, ctypes.c_int64, c_vp, ctypes.c_int64, ctypes.c_int64,
+                                              ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, c_vp,
+                                              c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "feq_expert_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FeqExpertLinearArgs), ctypes.c_int32]),
+    "feq_expert_linear_fwd": (ctypes.c_int, [ctypes.POINTER(FeqExpertLinearArgs), c_vp, ctypes.c_size_t, c_vp]),
+    "feq_expert_linear_bwd": (ctypes.c_int, [ctypes.POINTER(FeqExpertLinearArgs), c_vp, ctypes.c_size_t, c_vp]),
 }
 
 _lock = threading.Lock()

@@ -144,3 +144,21 @@ class SeparableEquivariantLayerNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"nscalar={self.nscalar}, nhigher={self.nhigher}"
+
+
+class InvariantLayerNorm(nn.LayerNorm):
+    """LayerNorm over the last dimension of invariant features (no counterpart in the reference), native
+    forward and backward on the GPU (csrc/feq_layernorm.cu); parameters as ``nn.LayerNorm`` holds
+    them, PyTorch's own on the CPU.  float32, bfloat16 or float16."""
+
+    def __init__(self, width: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True) -> None:
+        super().__init__(int(width), eps=eps, elementwise_affine=elementwise_affine, bias=bias)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not x.is_cuda:
+            return super().forward(x)
+        if x.shape[-1:] != self.normalized_shape:
+            raise ValueError(f"last dimension must be {self.normalized_shape[0]}; got {tuple(x.shape)}")
+        from ..cuda.token_autograd import layer_norm
+
+        return layer_norm(x, self.weight, self.bias, self.eps)

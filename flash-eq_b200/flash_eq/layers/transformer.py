@@ -16,6 +16,7 @@ from ..graph import Graph
 from ..partition import PartitionedGraph
 from ..representations import Repr, WignerDBasis
 from .attention import EquivariantAttention
+from .experts import EquivariantExperts
 from .gating import EquivariantGating
 from .linear import EquivariantLinear
 from .norm import SeparableEquivariantLayerNorm
@@ -48,13 +49,17 @@ class DropPath(nn.Module):
 
 
 class EquivariantTransformerBlock(nn.Module):
-    """norm -> attention (+ residual) -> norm -> gated MLP (+ residual)."""
+    """norm -> attention (+ residual) -> norm -> gated MLP (+ residual).
+
+    ``num_experts`` > 0 (no counterpart in the reference) replaces the gated MLP by a mixture of
+    that many experts, ``expert_top_k`` of them per node (``EquivariantExperts``)."""
 
     def __init__(self, in_repr: Repr, out_repr: Repr, num_heads: int = 1, num_bins: int = 100, rank: int = 4,
                  hidden_dim: int = 64, min_dist: float = 0.0, max_dist: float = 10.0, log_bins: bool = False,
                  mlp_ratio: int = 2, dropout: float = 0.0, drop_path: float = 0.0,
                  layer_scale_init: float | None = 1e-4, use_gating: bool = True, use_s2_activation: bool = False,
-                 s2_precision: int = 47, distance_decay_scale: float | None = None) -> None:
+                 s2_precision: int = 47, distance_decay_scale: float | None = None, num_experts: int = 0,
+                 expert_top_k: int = 2) -> None:
         super().__init__()
         if use_s2_activation:
             raise NotImplementedError(
@@ -69,10 +74,16 @@ class EquivariantTransformerBlock(nn.Module):
                                          log_bins=log_bins, dropout=dropout, reduce="sum",
                                          distance_decay_scale=distance_decay_scale)
         self.norm2 = SeparableEquivariantLayerNorm(out_repr)
-        hidden = Repr(lvals=out_repr.lvals, mult=out_repr.mult * mlp_ratio)
-        self.mlp_up = EquivariantLinear(out_repr, hidden, bias=True)
-        self.mlp_act: nn.Module = EquivariantGating(hidden) if use_gating else nn.Identity()
-        self.mlp_down = EquivariantLinear(hidden, out_repr, bias=True)
+        self.experts: EquivariantExperts | None = None
+        if num_experts > 0:
+            if not use_gating:
+                raise ValueError("use_gating=False has no meaning with num_experts > 0: the experts are gated")
+            self.experts = EquivariantExperts(out_repr, num_experts, top_k=expert_top_k, mlp_ratio=mlp_ratio)
+        else:
+            hidden = Repr(lvals=out_repr.lvals, mult=out_repr.mult * mlp_ratio)
+            self.mlp_up = EquivariantLinear(out_repr, hidden, bias=True)
+            self.mlp_act: nn.Module = EquivariantGating(hidden) if use_gating else nn.Identity()
+            self.mlp_down = EquivariantLinear(hidden, out_repr, bias=True)
         self.layer_scale_attn = (LayerScale(layer_scale_init) if layer_scale_init is not None
                                  and self._use_attn_residual else nn.Identity())
         self.layer_scale_mlp = LayerScale(layer_scale_init) if layer_scale_init is not None else nn.Identity()
@@ -92,7 +103,8 @@ class EquivariantTransformerBlock(nn.Module):
             x = self._residual(node_features, attn_out, self.layer_scale_attn)
         else:
             x = attn_out
-        mlp_out = self.mlp_down(self.mlp_act(self.mlp_up(self.norm2(x))))
+        h = self.norm2(x)
+        mlp_out = self.experts(h) if self.experts is not None else self.mlp_down(self.mlp_act(self.mlp_up(h)))
         return self._residual(x, mlp_out, self.layer_scale_mlp)
 
     def extra_repr(self) -> str:
@@ -106,7 +118,8 @@ class EquivariantTransformer(nn.Module):
                  num_bins: int = 100, rank: int = 4, hidden_dim: int = 64, min_dist: float = 0.0,
                  max_dist: float = 10.0, log_bins: bool = False, mlp_ratio: int = 2, dropout: float = 0.0,
                  drop_path: float = 0.0, layer_scale_init: float | None = 1e-4, use_s2_activation: bool = False,
-                 s2_precision: int = 47, distance_decay_scale: float | None = None) -> None:
+                 s2_precision: int = 47, distance_decay_scale: float | None = None, num_experts: int = 0,
+                 expert_top_k: int = 2) -> None:
         super().__init__()
         self.in_repr, self.hidden_repr, self.out_repr = in_repr, hidden_repr, out_repr
         self.num_layers = num_layers
@@ -123,7 +136,7 @@ class EquivariantTransformer(nn.Module):
                 hidden_dim=hidden_dim, min_dist=min_dist, max_dist=max_dist, log_bins=log_bins,
                 mlp_ratio=mlp_ratio, dropout=dropout, drop_path=rates[i], layer_scale_init=layer_scale_init,
                 use_s2_activation=use_s2_activation, s2_precision=s2_precision,
-                distance_decay_scale=distance_decay_scale))
+                distance_decay_scale=distance_decay_scale, num_experts=num_experts, expert_top_k=expert_top_k))
         self.final_norm = SeparableEquivariantLayerNorm(out_repr)
 
     def forward(self, coordinates: torch.Tensor, node_features: torch.Tensor, graph: Graph) -> torch.Tensor:

@@ -61,7 +61,8 @@ enum feq_status_code {
 const char *feq_status_string(int status);
 /* 2: FeqAttnArgs gained k / num_src_nodes (partitioned graphs).
  * 3: attention / pooling backward entry points, node-level operators.
- * 4: feq_set_wait_limit_ns; the separable (low-rank) edgewise entry point. */
+ * 4: feq_set_wait_limit_ns; the separable (low-rank) edgewise entry point.
+ * 5: layer norm, expert routing and expert linear. */
 int feq_abi_version(void);
 /* Limit, in nanoseconds, of every pipeline wait of the tensor-core kernels launched
  * after this call (no counterpart in the reference).  A wait that runs past it ends
@@ -538,6 +539,90 @@ int feq_radius_fill(const float *xyz, const int64_t *batch, int64_t num_points, 
                     float x0, float y0, float z0, const int64_t *offsets, int64_t num_edges, int64_t *src,
                     int64_t *dst, const void *workspace, size_t workspace_bytes, void *pair_workspace,
                     size_t pair_workspace_bytes, feq_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Layer norm and mixture-of-experts operators on token features (no counterpart in the
+ * reference).  Element types: FEQ_DTYPE_*; sums, statistics and routing weights are float32 and
+ * a value is rounded to a 16-bit type once, when it is stored.  Strides are in elements; the
+ * last dimension of every tensor is contiguous.
+ * ------------------------------------------------------------------------ */
+#define FEQ_DTYPE_F32 0
+#define FEQ_DTYPE_BF16 1
+#define FEQ_DTYPE_F16 2
+
+/* y = (x - mean) * rstd * weight + bias over rows of `width` elements; weight / bias (width) may
+ * be NULL and are in x's type, or float32 with param_f32 != 0.  mean / rstd (rows, float32) are
+ * kept for the backward; both NULL when it is not needed.  y is contiguous. */
+int feq_layer_norm_fwd(const void *x, int64_t rows, int64_t x_stride, int32_t width, int32_t dtype, const void *weight,
+                       const void *bias, int32_t param_f32, float eps, void *y, float *mean, float *rstd,
+                       feq_stream_t stream);
+/* grad_x (contiguous), grad_weight and grad_bias of the above; any of the three may be NULL.  The
+ * parameters' gradients are summed in a fixed order through the workspace. */
+size_t feq_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t width);
+int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, const void *x, int64_t rows, int64_t x_stride,
+                       int32_t width, int32_t dtype, const void *weight, int32_t param_f32, const float *mean,
+                       const float *rstd, void *grad_x, void *grad_weight, void *grad_bias, void *workspace,
+                       size_t workspace_bytes, feq_stream_t stream);
+
+/* Routing: per token the top_k largest of its num_experts logits (equal logits: the lower expert
+ * first; -inf is never chosen), ids (tokens, top_k) with -1 where a choice is missing; weights
+ * (tokens, top_k) = the softmax over the chosen logits (normalize != 0) or over all of them, 0
+ * where a choice is missing; slots (tokens, top_k) = the place of every (token, choice) pair in the
+ * stable order by expert, pairs without an expert last; offsets (num_experts + 1) = the first place
+ * of each expert, offsets[num_experts] = the number of pairs that have one.  NaN counts as the
+ * largest logit.  num_experts <= 512, top_k <= 32, tokens * top_k < 2^31. */
+size_t feq_expert_route_workspace_bytes(int64_t tokens, int32_t top_k, int32_t num_experts);
+int feq_expert_route(const void *logits, int64_t tokens, int64_t stride, int32_t num_experts, int32_t top_k,
+                     int32_t dtype, int32_t normalize, int32_t *ids, float *weights, int32_t *slots, int32_t *offsets,
+                     void *workspace, size_t workspace_bytes, feq_stream_t stream);
+/* grad_logits (tokens, num_experts), contiguous, in the logits' type. */
+int feq_expert_route_bwd(const void *logits, int64_t tokens, int64_t stride, int32_t num_experts, int32_t top_k,
+                         int32_t dtype, int32_t normalize, const int32_t *ids, const float *weights,
+                         const float *grad_weights, void *grad_logits, feq_stream_t stream);
+/* sorted[slots[n, j]] = x[n], 0 for pairs without an expert; sorted (tokens * top_k, width). */
+int feq_expert_dispatch(const void *x, int64_t tokens, int64_t x_stride, int64_t width, int32_t dtype, int32_t top_k,
+                        int32_t num_experts, const int32_t *slots, const int32_t *offsets, void *sorted,
+                        feq_stream_t stream);
+/* out[n] = sum_j weights[n, j] sorted[slots[n, j]] over the pairs that have an expert (weights NULL:
+ * 1, which is the gradient of the dispatch); out (tokens, width). */
+int feq_expert_combine(const void *sorted, int64_t sorted_stride, int64_t tokens, int64_t width, int32_t dtype,
+                       int32_t top_k, int32_t num_experts, const int32_t *slots, const int32_t *offsets,
+                       const float *weights, void *out, feq_stream_t stream);
+/* grad_sorted[slots[n, j]] = weights[n, j] grad_out[n] (0 without an expert) and
+ * grad_weights[n, j] = <grad_out[n], sorted[slots[n, j]]>. */
+int feq_expert_combine_bwd(const void *grad_out, int64_t grad_stride, const void *sorted, int64_t sorted_stride,
+                           int64_t tokens, int64_t width, int32_t dtype, int32_t top_k, int32_t num_experts,
+                           const int32_t *slots, const int32_t *offsets, const float *weights, void *grad_sorted,
+                           float *grad_weights, feq_stream_t stream);
+
+/* The experts' linear maps on rows sorted by expert: x (rows, dim, c_in) with dim = sum(2 l + 1)
+ * over lvals (lvals = {0}: plain rows), weight (num_experts, n_lvals, c_out, c_in), bias
+ * (num_experts, scalars, c_out) on the l = 0 components or NULL; out (rows, dim, c_out)
+ * contiguous.  Rows of expert e are offsets[e] .. offsets[e + 1) (device, int32); rows from
+ * offsets[num_experts] on give zeros.  All tensors have the type `dtype`.
+ * The backward fills those of grad_x (rows, dim, c_in), grad_weight and grad_bias that are not
+ * NULL.  status (may be NULL): 2 when a tensor-core wait timed out (result invalid).
+ * num_experts <= 512, rows < 2^31. */
+typedef struct {
+    const void *x;
+    int64_t x_row_stride, x_comp_stride;
+    const void *weight, *bias;
+    const int32_t *offsets;
+    int64_t rows;
+    const int32_t *lvals;
+    int32_t n_lvals, num_experts, c_in, c_out, dtype;
+    void *out;
+    const void *grad_out;
+    int64_t grad_row_stride, grad_comp_stride;
+    void *grad_x, *grad_weight, *grad_bias;
+    int32_t *status;
+} FeqExpertLinearArgs;
+/* 0: the shape is not served. */
+size_t feq_expert_linear_workspace_bytes(const FeqExpertLinearArgs *args, int32_t backward);
+int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *workspace, size_t workspace_bytes,
+                          feq_stream_t stream);
+int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *workspace, size_t workspace_bytes,
+                          feq_stream_t stream);
 
 #ifdef __cplusplus
 }
