@@ -6,161 +6,750 @@
 //   gb[e, s]    = sum over rows r of e of gy[r, component of scalar s]
 //
 // Rows of expert e are offsets[e] .. offsets[e + 1); rows from offsets[experts] on belong to none and
-// give zeros.  The offsets stay on the device.
+// give zeros.  The offsets stay on the device: every kernel lays out its own work from them.
+//
+// The three products are one persistent tcgen05 kernel (gemm_kernel), a CTA per SM, 128 x BN tiles:
+//   warp 0      loads: tensor-map copies of 64-deep operand chunks into a ring (no multicast)
+//   warp 1      one thread issues tcgen05.mma kind::f16 into one of two TMEM accumulators
+//   warps 2..5  epilogue: tcgen05.ld, + bias, through shared memory to row-contiguous stores, while
+//               the next tile's products run
+//   warp 6      (gW only) passes every chunk on to warp 1, and in the last chunk of an expert's rows
+//               first zeroes the rows that belong to the next expert, in both operands
+// The contraction runs over channels in y and gx and over rows in gW; an operand whose channels
+// are not the contraction is read MN-major (the shared-memory tile as the copy leaves it), so
+// nothing is transposed.  bfloat16 and float16 operands are read where they lie when a tensor
+// map can describe them (16-byte addresses and strides), else from a packed copy.  float32: each
+// operand is packed as three bfloat16 planes whose sum is the value to 24 bits, and six products
+// (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave an error of 2^-24 of the terms; an infinite
+// input gives NaN in the sums that hold it.  The tensor cores cut their running sum off at 24 bits
+// instead of rounding it, which adds about 2e-8 of the sum per product: so hi hi has an accumulator of
+// its own (the five others add to a sum 2^-8 as large), and after kSegment chunks the epilogue
+// adds both to float32 registers (measured against float64 at K = 576: 3.9e-6 with one accumulator).
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "feq_sm100.cuh"
 #include "feq_token.cuh"
 
 namespace feq {
 namespace elin {
 
 using namespace token;
+using namespace sm100;
 
 constexpr int kMaxExperts = 512;
-constexpr int kT = 64;                        // tile edge
+constexpr int BM = 128, BK = 64;
+constexpr int kThreads = 7 * 32;
+constexpr uint32_t kBox = 64 * 128;                 // bytes of a 64-row, 64-channel box
+constexpr int kMaxStages = 8;
+constexpr int kSegment = 4;                         // chunks a float32 accumulator runs over
+constexpr int kLongestPart = 65536;                 // terms of one 16-bit sum over rows
+constexpr int kStageLd = 36;                        // floats per row of the epilogue's staging block
+constexpr uint32_t kStaging = 4 * 32 * kStageLd * 4;
+constexpr uint32_t kSmemLimit = 227 * 1024 - 6 * 1024;   // dynamic part; barriers and prefixes are static
+
+enum Mode { kForward = 0, kGradX = 1, kGradW = 2 };
 
 // Components of a row: which weight they use, and which bias (-1: none).
 struct Comps {
     int dim, reps, scalars;
-    int8_t rep[kMaxDim], scalar[kMaxDim];
+    int16_t first[kMaxIrreps + 1];                  // first component of each irrep
+    int8_t scalar_of[kMaxIrreps];                   // scalar index of an l = 0 irrep, else -1
+    int8_t rep[kMaxDim];
 };
 
-struct Args {
-    const void *x, *w, *b, *gy;               // b in the weights' type
-    void *y, *gx, *gw, *gb;
-    int64_t rows, x_row, x_comp, gy_row, gy_comp;   // strides in elements; channels are contiguous
-    int experts, cin, cout;
+struct Params {
     const int32_t *offsets;
+    int experts;
+    int64_t rows;
+    int J, K;                // row modes: output channels, contraction; gW: rows (c_out) and columns (c_in)
+    int out_dtype, bias_dtype;
+    void *out;               // gW: the gradient, or (chunk_rows > 0 and split) float32 partial sums
+    const void *bias;
+    uint32_t idesc;
+    int stages;
+    int chunk_rows;          // gW: rows of one contraction part (a multiple of 64)
+    int split;               // gW: parts go to partial sums, joined by join_kernel
+    int32_t *status;
+    uint64_t wait_ns;
 };
 
-// offsets as the kernels use them: never decreasing and within the rows.
-__device__ __forceinline__ void load_offsets(const Args &a, int32_t *off) {
-    if (threadIdx.x == 0) {
-        int32_t at = 0;
-        for (int e = 0; e <= a.experts; e++) {
-            const int32_t v = a.offsets[e];
-            if (e > 0) at = v < at ? at : (v > a.rows ? (int32_t)a.rows : v);
-            off[e] = at;
+// Shared-memory descriptor, MN-major operand with 128-byte swizzle: boxes of 64 k rows x 64 mn
+// (128 B a row), 8 k rows = 1024 B (SBO), the next 64 mn in the next box (LBO).
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+    d |= (uint64_t)(kBox >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// off[e] (never decreasing, within the rows) and pre[e] = first unit of expert e, where an expert
+// has `units(rows)` of them; one warp, 32 experts at a time.
+template <typename F>
+__device__ __forceinline__ void lay_out(const int32_t *offsets, int experts, int64_t rows, int32_t *off, int32_t *pre,
+                                        F units) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int32_t seen = 0;
+        for (int e0 = 0; e0 <= experts; e0 += 32) {
+            const int e = e0 + lane;
+            int32_t v = 0;
+            if (e > 0 && e <= experts) v = (int32_t)min64(max64(offsets[e], 0), rows);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v = max(v, u);
+            }
+            v = max(v, seen);
+            if (e <= experts) off[e] = v;
+            seen = __shfl_sync(0xffffffffu, v, 31);
         }
+        __syncwarp();
+        int32_t base = 0;
+        for (int e0 = 0; e0 < experts; e0 += 32) {
+            const int e = e0 + lane;
+            const int32_t n = e < experts ? units(off[e + 1] - off[e]) : 0;
+            int32_t s = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            if (e < experts) pre[e] = base + s - n;
+            base += __shfl_sync(0xffffffffu, s, 31);
+        }
+        if (lane == 0) pre[experts] = base;
     }
     __syncthreads();
 }
 
-// Tile `tile` of the row tiles of all experts (each expert's rows in tiles of kT, then the rows
-// that belong to none): expert (a.experts for none) and first and last row; false past the end.
-__device__ __forceinline__ bool find_tile(const Args &a, const int32_t *off, int tile, int &e, int64_t &r0, int64_t &r1) {
-    for (e = 0; e <= a.experts; e++) {
-        const int64_t lo = off[e], hi = e == a.experts ? a.rows : off[e + 1];
-        const int n = (int)((hi - lo + kT - 1) / kT);
-        if (tile < n) {
-            r0 = lo + (int64_t)tile * kT;
-            r1 = min64(r0 + kT, hi);
-            return true;
-        }
-        tile -= n;
+// One unit of work of a CTA.
+struct Tile {
+    int e, p, n0;            // row modes: expert, component, first output channel; gW: expert, irrep, first c_in
+    int m0;                  // gW: first c_out
+    int64_t r0, r1;          // rows
+    int nk;                  // contraction chunks
+    int part;                // gW: index of the partial sum
+};
+
+template <int MODE, int BN>
+struct Walk {
+    const Params &a;
+    const Comps &c;
+    const int32_t *off, *pre;
+    int e = 0, tiles_n, tiles_m;
+    int64_t t, total;
+    __device__ Walk(const Params &a_, const Comps &c_, const int32_t *off_, const int32_t *pre_)
+        : a(a_), c(c_), off(off_), pre(pre_) {
+        tiles_n = ((MODE == kGradW ? a.K : a.J) + BN - 1) / BN;
+        tiles_m = MODE == kGradW ? (a.J + BM - 1) / BM : 1;
+        total = (int64_t)pre[a.experts] * (MODE == kGradW ? c.reps * tiles_m : c.dim) * tiles_n;
+        t = blockIdx.x;
     }
-    return false;
+    __device__ bool next(Tile &q) {
+        if (t >= total) return false;
+        int64_t u = t;
+        t += gridDim.x;
+        const int nt = (int)(u % tiles_n);
+        u /= tiles_n;
+        q.n0 = nt * BN;
+        if (MODE == kGradW) {
+            q.m0 = (int)(u % tiles_m) * BM;
+            u /= tiles_m;
+        } else {
+            q.m0 = 0;
+        }
+        const int inner = MODE == kGradW ? c.reps : c.dim;
+        q.p = (int)(u % inner);
+        const int unit = (int)(u / inner);
+        while (pre[e + 1] <= unit) e++;
+        q.e = e;
+        const int span = MODE == kGradW ? a.chunk_rows : BM;
+        q.r0 = off[e] + (int64_t)(unit - pre[e]) * span;
+        q.r1 = min64(q.r0 + span, off[e + 1]);
+        q.part = unit * c.reps + q.p;
+        if (MODE == kGradW)
+            q.nk = (int)((q.r1 - q.r0 + BK - 1) / BK) * (c.first[q.p + 1] - c.first[q.p]);
+        else
+            q.nk = (a.K + BK - 1) / BK;
+        return true;
+    }
+};
+
+template <int MODE, int PLANES, int BN>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+            const __grid_constant__ Params a, const __grid_constant__ Comps c) {
+    constexpr bool kAmn = MODE == kGradW, kBmn = MODE != kForward;
+    constexpr uint32_t kA = BM * 128, kB = BN * 128;           // one plane of a chunk
+    constexpr uint32_t kStage = PLANES * (kA + kB);
+    constexpr uint32_t kAcc = PLANES == 3 ? 2 * BN : BN;       // TMEM columns of one accumulator (pair)
+    constexpr uint32_t kCols = 2 * kAcc;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], fixed[kMaxStages], t_full[2], t_empty[2], drain;
+    __shared__ uint32_t tmem_s;
+    __shared__ int abort_s;
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float *staging = reinterpret_cast<float *>(smem + (size_t)a.stages * kStage);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+            mbar_init(&fixed[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&t_full[b], 1);
+            mbar_init(&t_empty[b], 4);
+        }
+        mbar_init(&drain, 1);
+        abort_s = 0;
+        fence_mbar_init();
+        prefetch_tmap(&amap);
+        prefetch_tmap(&bmap);
+    }
+    lay_out(a.offsets, a.experts, a.rows, off, pre, [&](int32_t n) {
+        if (MODE != kGradW) return (n + BM - 1) / BM;
+        // an expert without rows still has its gradient (zeros) to write when nothing joins parts
+        return n == 0 ? (a.split ? 0 : 1) : (n + a.chunk_rows - 1) / a.chunk_rows;
+    });
+    if (warp == 0) {
+        tmem_alloc(&tmem_s, kCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    volatile int *abort_flag = &abort_s;
+    Walk<MODE, BN> walk(a, c, off, pre);
+    Tile q;
+
+    if (warp == 0) {
+        // ---------------- loads ----------------
+        if (lane == 0) {
+            uint32_t u = 0;
+            bool ok = true;
+            while (ok && !*abort_flag && walk.next(q)) {
+                const int blocks = MODE == kGradW ? (int)((q.r1 - q.r0 + BK - 1) / BK) : 0;
+                for (int kc = 0; kc < q.nk; kc++, u++) {
+                    const int s = (int)(u % a.stages);
+                    if (u >= (uint32_t)a.stages && !mbar_wait(&empty[s], ((u / a.stages) - 1) & 1u, abort_flag, a.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *st = smem + (size_t)s * kStage;
+                    mbar_arrive_expect_tx(&full[s], kStage);
+#pragma unroll
+                    for (int pl = 0; pl < PLANES; pl++) {
+                        uint8_t *sa = st + pl * kA, *sb = st + PLANES * kA + pl * kB;
+                        if (MODE == kGradW) {
+                            const int p = c.first[q.p] + kc / blocks, r = (int)q.r0 + (kc % blocks) * BK;
+#pragma unroll
+                            for (int i = 0; i < BM / 64; i++) tma_load_4d(sa + i * kBox, &amap, q.m0 + i * 64, p, r, pl, &full[s]);
+#pragma unroll
+                            for (int i = 0; i < BN / 64; i++) tma_load_4d(sb + i * kBox, &bmap, q.n0 + i * 64, p, r, pl, &full[s]);
+                        } else {
+                            tma_load_4d(sa, &amap, kc * BK, q.p, (int)q.r0, pl, &full[s]);
+                            const int wi = q.e * c.reps + c.rep[q.p];
+                            if (kBmn) {
+#pragma unroll
+                                for (int i = 0; i < BN / 64; i++)
+                                    tma_load_4d(sb + i * kBox, &bmap, q.n0 + i * 64, kc * BK, wi, pl, &full[s]);
+                            } else {
+                                tma_load_4d(sb, &bmap, kc * BK, q.n0, wi, pl, &full[s]);
+                            }
+                        }
+                    }
+                }
+            }
+            // every copy issued has landed before the CTA leaves
+            for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
+                mbar_wait_drain(&full[v % a.stages], (v / a.stages) & 1u);
+        }
+    } else if (warp == 1) {
+        // ---------------- products ----------------
+        if (lane == 0) {
+            uint32_t u = 0, used = 0;
+            bool ok = true;
+            while (ok && !*abort_flag && walk.next(q)) {
+                uint32_t d = 0;
+                int buf = 0;
+                for (int kc = 0; kc < q.nk; kc++, u++) {
+                    const bool first = PLANES == 3 ? kc % kSegment == 0 : kc == 0;
+                    if (first) {
+                        buf = (int)(used & 1);
+                        if (used >= 2 && !mbar_wait(&t_empty[buf], ((used >> 1) - 1) & 1u, abort_flag, a.wait_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        used++;
+                        tc_fence_after();
+                        d = tmem + (uint32_t)buf * kAcc;
+                    }
+                    const int s = (int)(u % a.stages);
+                    uint64_t *ready = MODE == kGradW ? &fixed[s] : &full[s];
+                    if (!mbar_wait(ready, (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + (size_t)s * kStage), sb = sa + PLANES * kA;
+#pragma unroll
+                    for (int ks = 0; ks < BK / 16; ks++) {
+                        const uint32_t ao = sa + (kAmn ? ks * 2048 : ks * 32), bo = sb + (kBmn ? ks * 2048 : ks * 32);
+                        // planes: hi hi, then (three planes) the five smaller products
+                        constexpr int kPairs = PLANES == 1 ? 1 : 6;
+                        constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+#pragma unroll
+                        for (int i = 0; i < kPairs; i++) {
+                            const uint32_t aa = ao + pa[i] * kA, bb = bo + pb[i] * kB;
+                            umma_f16(i == 0 ? d : d + BN, kAmn ? smem_desc_mn(aa) : smem_desc_sw128(aa),
+                                     kBmn ? smem_desc_mn(bb) : smem_desc_sw128(bb), a.idesc,
+                                     first && ks == 0 && i <= 1 ? 0u : 1u);
+                        }
+                    }
+                    umma_commit(&empty[s]);
+                    if (kc == q.nk - 1 || (PLANES == 3 && kc % kSegment == kSegment - 1)) umma_commit(&t_full[buf]);
+                }
+            }
+            umma_commit(&drain);
+            mbar_wait_drain(&drain, 0);
+        }
+    } else if (warp < 6) {
+        // ---------------- epilogue ----------------
+        const int quad = warp & 3;
+        float *st = staging + quad * 32 * kStageLd;
+        const int es = a.out_dtype == FEQ_DTYPE_F32 ? 4 : 2;
+        const int ld = MODE == kGradW ? a.K : a.J, cols = ld;
+        const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)ld * es) & 15) == 0;
+        if (MODE != kGradW) {
+            // rows that belong to no expert: one contiguous range of zeros
+            const int64_t lo = (int64_t)off[a.experts] * c.dim * ld * es, hi = a.rows * c.dim * (int64_t)ld * es;
+            uint8_t *o = static_cast<uint8_t *>(a.out);
+            const int64_t step = (int64_t)gridDim.x * 128 * es;
+            for (int64_t i = lo + ((int64_t)blockIdx.x * 128 + threadIdx.x - 64) * es; i < hi; i += step) {
+                if (es == 4)
+                    *reinterpret_cast<float *>(o + i) = 0.0f;
+                else
+                    *reinterpret_cast<uint16_t *>(o + i) = 0;
+            }
+        }
+        uint32_t used = 0;
+        while (!*abort_flag && walk.next(q)) {
+            float acc[PLANES == 3 ? BN : 1];
+            bool ok = true;
+            if (PLANES == 3) {
+#pragma unroll
+                for (int i = 0; i < (PLANES == 3 ? BN : 1); i++) acc[i] = 0.0f;
+                for (int kc = 0; kc < q.nk; kc += kSegment, used++) {
+                    const int buf = (int)(used & 1);
+                    if (!mbar_wait(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)buf * kAcc;
+#pragma unroll
+                    for (int c0 = 0; c0 < (PLANES == 3 ? BN : 0); c0 += 32) {
+                        uint32_t u[32], w[32];
+                        tmem_ld32(t + c0, u);
+                        tmem_ld32(t + BN + c0, w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) acc[c0 + i] += __uint_as_float(u[i]) + __uint_as_float(w[i]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&t_empty[buf]);
+                }
+            } else if (q.nk > 0) {
+                ok = mbar_wait(&t_full[used & 1], (used >> 1) & 1u, abort_flag, a.wait_ns);
+                tc_fence_after();
+            }
+            if (!ok) break;
+            const int sc = MODE == kForward && a.bias ? c.scalar_of[c.rep[q.p]] : -1;
+            // row i of this warp's 32 rows: valid below `live`, at out + i * pitch
+            int live;
+            int64_t at, pitch;
+            if (MODE == kGradW) {
+                live = min(32, max(0, a.J - q.m0 - quad * 32));
+                const int64_t unit = a.split ? q.part : (int64_t)q.e * c.reps + q.p;
+                at = (unit * a.J + q.m0 + quad * 32) * ld;
+                pitch = ld;
+            } else {
+                live = (int)max64(0, min64(32, q.r1 - q.r0 - quad * 32));
+                at = ((q.r0 + quad * 32) * c.dim + q.p) * (int64_t)ld;
+                pitch = (int64_t)c.dim * ld;
+            }
+#pragma unroll (PLANES == 3 ? BN / 32 : 1)
+            for (int c0 = 0; c0 < BN; c0 += 32) {
+                if (q.n0 + c0 >= cols) break;
+                uint32_t v[32];
+                if (PLANES == 3) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(acc[PLANES == 3 ? c0 + i : 0]);
+                } else if (q.nk > 0) {
+                    tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (used & 1) * kAcc + c0, v);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = 0u;
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<uint4 *>(st + lane * kStageLd + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                __syncwarp();
+                auto bias_at = [&](int col) -> float {
+                    if (sc < 0 || col >= cols) return 0.0f;
+                    const int64_t i = ((int64_t)q.e * c.scalars + sc) * a.J + col;
+                    return a.bias_dtype == FEQ_DTYPE_F32 ? static_cast<const float *>(a.bias)[i]
+                           : a.bias_dtype == FEQ_DTYPE_BF16 ? to_f32(static_cast<const __nv_bfloat16 *>(a.bias)[i])
+                                                            : to_f32(static_cast<const __half *>(a.bias)[i]);
+                };
+                if (vec && es == 4) {
+                    const int cc = (lane & 7) * 4, col = q.n0 + c0 + cc;
+                    const float b0 = bias_at(col), b1 = bias_at(col + 1), b2 = bias_at(col + 2), b3 = bias_at(col + 3);
+                    float *o = static_cast<float *>(a.out) + at + col;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int row = i * 4 + (lane >> 3);
+                        float4 f = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc);
+                        f.x += b0;
+                        f.y += b1;
+                        f.z += b2;
+                        f.w += b3;
+                        if (row < live && col < cols) *reinterpret_cast<float4 *>(o + row * pitch) = f;
+                    }
+                } else if (vec) {
+                    const int cc = (lane & 3) * 8, col = q.n0 + c0 + cc;
+                    float b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) b[i] = bias_at(col + i);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int row = i * 8 + (lane >> 2);
+                        const float4 f = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc);
+                        const float4 g = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc + 4);
+                        const float w[8] = {f.x + b[0], f.y + b[1], f.z + b[2], f.w + b[3],
+                                            g.x + b[4], g.y + b[5], g.z + b[6], g.w + b[7]};
+                        if (row < live && col < cols) {
+                            if (a.out_dtype == FEQ_DTYPE_BF16) {
+                                Pack<__nv_bfloat16, 8> o;
+#pragma unroll
+                                for (int k = 0; k < 8; k++) o.v[k] = from_f32<__nv_bfloat16>(w[k]);
+                                *reinterpret_cast<Pack<__nv_bfloat16, 8> *>(static_cast<__nv_bfloat16 *>(a.out) + at +
+                                                                           row * pitch + col) = o;
+                            } else {
+                                Pack<__half, 8> o;
+#pragma unroll
+                                for (int k = 0; k < 8; k++) o.v[k] = from_f32<__half>(w[k]);
+                                *reinterpret_cast<Pack<__half, 8> *>(static_cast<__half *>(a.out) + at + row * pitch + col) = o;
+                            }
+                        }
+                    }
+                } else {
+                    const int col = q.n0 + c0 + lane;
+                    const float b = bias_at(col);
+                    if (col < cols) {
+                        for (int row = 0; row < live; row++) {
+                            const float w = st[row * kStageLd + lane] + b;
+                            const int64_t o = at + row * pitch + col;
+                            if (a.out_dtype == FEQ_DTYPE_F32)
+                                static_cast<float *>(a.out)[o] = w;
+                            else if (a.out_dtype == FEQ_DTYPE_BF16)
+                                static_cast<__nv_bfloat16 *>(a.out)[o] = from_f32<__nv_bfloat16>(w);
+                            else
+                                static_cast<__half *>(a.out)[o] = from_f32<__half>(w);
+                        }
+                    }
+                }
+            }
+            if (PLANES == 1 && q.nk > 0) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&t_empty[used & 1]);
+                used++;
+            }
+        }
+    } else if (MODE == kGradW) {
+        // ---------------- rows of a chunk that belong to the next expert ----------------
+        uint32_t u = 0;
+        bool ok = true;
+        while (ok && !*abort_flag && walk.next(q)) {
+            const int blocks = (int)((q.r1 - q.r0 + BK - 1) / BK), live = (int)((q.r1 - q.r0) % BK);
+            for (int kc = 0; kc < q.nk; kc++, u++) {
+                const int s = (int)(u % a.stages);
+                if (!mbar_wait(&full[s], (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
+                    ok = false;
+                    break;
+                }
+                if (live != 0 && kc % blocks == blocks - 1) {
+                    // a k row is 128 bytes of every box; the swizzle moves data within a row only
+                    uint8_t *st = smem + (size_t)s * kStage;
+                    const int per = (BK - live) * 8;                 // 16-byte pieces of a box
+                    for (int i = lane; i < per * (int)(kStage / kBox); i += 32) {
+                        const int box = i / per, j = i - box * per;
+                        *reinterpret_cast<uint4 *>(st + box * kBox + live * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&fixed[s]);
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kCols);
+    }
+    if (threadIdx.x == 0 && abort_s) set_status(a.status, 2);
 }
 
-// C[r, j] = sum_k A[r, k] B[j * bj + k * bk] (+ bias[j]) for one row tile, 64 columns, one component.
+// gW = the sum of an expert's partial sums, in their order.
 template <typename T>
 __global__ void __launch_bounds__(256)
-rows_kernel(const Args a, const Comps c, const T *A, int64_t a_row, int64_t a_comp, int K, int J, int bj, int bk,
-            const T *bias, T *C) {
-    __shared__ int32_t off[kMaxExperts + 1];
-    __shared__ float As[kT][17], Bs[kT][17];
-    load_offsets(a, off);
-    int e;
-    int64_t r0, r1;
-    if (!find_tile(a, off, blockIdx.y, e, r0, r1)) return;
-    const int p = blockIdx.z, j0 = blockIdx.x * kT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    float acc[4][4] = {};
-    if (e < a.experts) {
-        const T *B = static_cast<const T *>(a.w) + ((int64_t)e * c.reps + c.rep[p]) * a.cin * a.cout;
-        for (int k0 = 0; k0 < K; k0 += 16) {
-            for (int i = threadIdx.x; i < kT * 16; i += 256) {
-                const int row = i >> 4, k = k0 + (i & 15);
-                As[row][i & 15] = r0 + row < r1 && k < K ? to_f32(A[(r0 + row) * a_row + p * a_comp + k]) : 0.0f;
-                Bs[row][i & 15] = j0 + row < J && k < K ? to_f32(B[(int64_t)(j0 + row) * bj + (int64_t)k * bk]) : 0.0f;
-            }
-            __syncthreads();
-            for (int k = 0; k < 16; k++)
-                for (int u = 0; u < 4; u++)
-                    for (int v = 0; v < 4; v++) acc[u][v] += As[ty * 4 + u][k] * Bs[tx * 4 + v][k];
-            __syncthreads();
-        }
+join_kernel(const float *__restrict__ part, const int32_t *offsets, int experts, int64_t rows, int chunk_rows, int reps,
+            int64_t size, T *__restrict__ out) {
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
+    lay_out(offsets, experts, rows, off, pre, [&](int32_t n) { return (n + chunk_rows - 1) / chunk_rows; });
+    const int e = blockIdx.y / reps, rep = blockIdx.y % reps;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+        float s = 0.0f;
+        for (int u = pre[e]; u < pre[e + 1]; u++) s += part[((int64_t)u * reps + rep) * size + i];
+        out[(int64_t)blockIdx.y * size + i] = from_f32<T>(s);
     }
-    for (int u = 0; u < 4; u++)
-        for (int v = 0; v < 4; v++) {
-            const int64_t r = r0 + ty * 4 + u;
-            const int j = j0 + tx * 4 + v;
-            if (r >= r1 || j >= J) continue;
-            float s = acc[u][v];
-            if (bias && e < a.experts && c.scalar[p] >= 0)
-                s += to_f32(bias[((int64_t)e * c.scalars + c.scalar[p]) * J + j]);
-            C[(r * c.dim + p) * J + j] = from_f32<T>(s);
-        }
 }
 
-// gW of one expert and irrep, a 64 x 64 tile (o, i).
+// gb of one expert and scalar: 32 columns a block, a warp per 32nd row, sums joined in warp order.
 template <typename T>
-__global__ void __launch_bounds__(256) weights_kernel(const Args a, const Comps c) {
-    __shared__ int32_t off[kMaxExperts + 1];
-    __shared__ float Gs[16][kT + 1], Xs[16][kT + 1];
-    load_offsets(a, off);
-    const int e = blockIdx.z / c.reps, rep = blockIdx.z % c.reps;
-    const int o0 = blockIdx.y * kT, i0 = blockIdx.x * kT, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const T *x = static_cast<const T *>(a.x), *g = static_cast<const T *>(a.gy);
-    float acc[4][4] = {}, total[4][4] = {};
-    for (int p = 0; p < c.dim; p++) {
-        if (c.rep[p] != rep) continue;
-        for (int64_t r0 = off[e]; r0 < off[e + 1]; r0 += 16) {
-            for (int i = threadIdx.x; i < kT * 16; i += 256) {
-                const int row = i >> 6, col = i & 63;
-                const bool live = r0 + row < off[e + 1];
-                Gs[row][col] = live && o0 + col < a.cout ? to_f32(g[(r0 + row) * a.gy_row + p * a.gy_comp + o0 + col]) : 0.0f;
-                Xs[row][col] = live && i0 + col < a.cin ? to_f32(x[(r0 + row) * a.x_row + p * a.x_comp + i0 + col]) : 0.0f;
-            }
-            __syncthreads();
-            for (int k = 0; k < 16; k++)
-                for (int u = 0; u < 4; u++)
-                    for (int v = 0; v < 4; v++) acc[u][v] += Gs[k][ty * 4 + u] * Xs[k][tx * 4 + v];
-            __syncthreads();
-            // sums of at most 256 rows are joined, so that a long sum keeps its last bits
-            if (((r0 - off[e]) & 255) == 240 || r0 + 16 >= off[e + 1])
-                for (int u = 0; u < 4; u++)
-                    for (int v = 0; v < 4; v++) {
-                        total[u][v] += acc[u][v];
-                        acc[u][v] = 0.0f;
-                    }
-        }
-    }
-    T *out = static_cast<T *>(a.gw) + (int64_t)blockIdx.z * a.cin * a.cout;
-    for (int u = 0; u < 4; u++)
-        for (int v = 0; v < 4; v++)
-            if (o0 + ty * 4 + u < a.cout && i0 + tx * 4 + v < a.cin)
-                out[(int64_t)(o0 + ty * 4 + u) * a.cin + i0 + tx * 4 + v] = from_f32<T>(total[u][v]);
-}
-
-// gb of one expert and scalar: a warp per 32 columns walks the expert's rows.
-template <typename T>
-__global__ void __launch_bounds__(1024) bias_kernel(const Args a, const Comps c) {
-    __shared__ int32_t off[kMaxExperts + 1];
+__global__ void __launch_bounds__(1024)
+bias_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const int32_t *offsets, int experts, int64_t rows,
+            int cout, const __grid_constant__ Comps c, T *__restrict__ out) {
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     __shared__ float sh[32][33];
-    load_offsets(a, off);
+    lay_out(offsets, experts, rows, off, pre, [](int32_t) { return 0; });
     const int e = blockIdx.y / c.scalars, sc = blockIdx.y % c.scalars;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, o = blockIdx.x * 32 + lane;
-    int p = 0;
-    while (c.scalar[p] != sc) p++;
+    int rep = 0;
+    while (c.scalar_of[rep] != sc) rep++;
+    const T *col = g + c.first[rep] * g_comp + o;
     float s = 0.0f;
-    if (o < a.cout)
-        for (int64_t r = off[e] + warp; r < off[e + 1]; r += 32)
-            s += to_f32(static_cast<const T *>(a.gy)[r * a.gy_row + p * a.gy_comp + o]);
+    if (o < cout)
+        for (int64_t r = off[e] + warp; r < off[e + 1]; r += 32) s += to_f32(col[r * g_row]);
     sh[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && o < a.cout) {
+    if (warp == 0 && o < cout) {
         float v = 0.0f;
         for (int k = 0; k < 32; k++) v += sh[k][lane];
-        static_cast<T *>(a.gb)[(int64_t)blockIdx.y * a.cout + o] = from_f32<T>(v);
+        out[(int64_t)blockIdx.y * cout + o] = from_f32<T>(v);
     }
+}
+
+// Rows (rows, dim, n) with strides of their own -> planes (PLANES, rows, dim, npad) of 16-bit values,
+// zeros from n to npad (a multiple of 8).  PLANES 3: float32 as three bfloat16 summing to it.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256)
+pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, int64_t row, int64_t comp,
+            uint16_t *__restrict__ dst) {
+    const int units = npad / 8;
+    const int64_t total = rows * dim * units, plane = rows * dim * (int64_t)npad;
+    const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uint64_t)row * sizeof(T) | (uint64_t)comp * sizeof(T)) & 15) == 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t rd = i / units;
+        const int k0 = (int)(i - rd * units) * 8;
+        const int64_t r = dim == 1 ? rd : rd / dim;
+        const T *s = src + r * row + (rd - r * dim) * comp + k0;
+        T v[8];
+        if (wide && k0 + 8 <= n) {
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<Pack<T, 4> *>(v) = *reinterpret_cast<const Pack<T, 4> *>(s);
+                *reinterpret_cast<Pack<T, 4> *>(v + 4) = *reinterpret_cast<const Pack<T, 4> *>(s + 4);
+            } else {
+                *reinterpret_cast<Pack<T, 8> *>(v) = *reinterpret_cast<const Pack<T, 8> *>(s);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; q++) v[q] = k0 + q < n ? s[q] : from_f32<T>(0.0f);
+        }
+        if constexpr (PLANES == 1) {
+            Pack<uint16_t, 8> o;
+#pragma unroll
+            for (int q = 0; q < 8; q++) o.v[q] = *reinterpret_cast<const uint16_t *>(&v[q]);
+            *reinterpret_cast<Pack<uint16_t, 8> *>(dst + i * 8) = o;
+        } else {
+            Pack<uint16_t, 8> o[3];
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+                const float x = v[q];
+                __nv_bfloat16 h = __float2bfloat16_rn(x);
+                if (__hisinf(h) && !isinf(x)) h = __float2bfloat16_rz(x);       // rounding up left the range
+                const bool finite = !isinf(x) && !isnan(x);
+                const float rest = finite ? x - __bfloat162float(h) : 0.0f;
+                const __nv_bfloat16 m = __float2bfloat16_rn(rest);
+                const __nv_bfloat16 l = __float2bfloat16_rn(rest - __bfloat162float(m));
+                o[0].v[q] = __bfloat16_as_ushort(h);
+                o[1].v[q] = __bfloat16_as_ushort(m);
+                o[2].v[q] = __bfloat16_as_ushort(l);
+            }
+#pragma unroll
+            for (int p = 0; p < 3; p++) *reinterpret_cast<Pack<uint16_t, 8> *>(dst + p * plane + i * 8) = o[p];
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+static int pad8(int n) { return (n + 7) & ~7; }
+
+// A (planes, rows, dim, n) 16-bit tensor as the kernels read it.
+struct Operand {
+    const void *base;
+    int64_t rows, row, comp, plane;       // strides in elements
+    int dim, n, planes;
+};
+
+// Map (n, dim, rows, planes); a box is 64 channels x `box_mid` x `box_rows` x 1.
+static int make_map(CUtensorMap *m, const Operand &o, int box_mid, int box_rows) {
+    EncodeFn fn = encode_fn();
+    if (!fn) {
+        record_error_text("cuTensorMapEncodeTiled is not available");
+        return FEQ_ERR_CUDA;
+    }
+    const int64_t comp = o.dim > 1 ? o.comp : pad8(o.n), row = o.rows > 1 ? o.row : o.dim * comp;
+    const int64_t plane = o.planes > 1 ? o.plane : o.rows * row;
+    cuuint64_t dims[4] = {(cuuint64_t)o.n, (cuuint64_t)o.dim, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
+    cuuint64_t strides[3] = {(cuuint64_t)comp * 2, (cuuint64_t)row * 2, (cuuint64_t)plane * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)box_mid, (cuuint32_t)box_rows, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(o.base), dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        record_error_text("cuTensorMapEncodeTiled refused an operand");
+        return FEQ_ERR_CUDA;
+    }
+    return FEQ_OK;
+}
+
+// Whether a tensor map describes (rows, dim, n) with these strides as it lies.
+static bool mappable(const void *p, int dtype, int64_t rows, int dim, int n, int64_t row, int64_t comp) {
+    if (dtype == FEQ_DTYPE_F32 || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+    // components and rows one after the other, without overlap; strides below 2^40 bytes
+    const int64_t most = (int64_t)1 << 30, inner = dim > 1 ? comp : pad8(n);
+    if (dim > 1 && (comp < n || comp % 8 || comp > most)) return false;
+    return rows == 1 || (row >= dim * inner && row % 8 == 0 && row <= most && rows * row < (int64_t)1 << 38);
+}
+
+static size_t packed_bytes(int dtype, int64_t rows, int dim, int n) {
+    return (size_t)rows * dim * pad8(n) * (dtype == FEQ_DTYPE_F32 ? 6 : 2);
+}
+
+// The operand as the kernels read it: where it lies, or packed into the workspace.
+static int operand(Operand *o, const void *p, int dtype, int64_t rows, int dim, int n, int64_t row, int64_t comp,
+                   WsCarver *ws, cudaStream_t s) {
+    o->rows = rows;
+    o->dim = dim;
+    o->n = n;
+    o->planes = 1;
+    if (mappable(p, dtype, rows, dim, n, row, comp)) {
+        o->base = p;
+        o->row = row;
+        o->comp = comp;
+        o->plane = 8;
+        return FEQ_OK;
+    }
+    const int np = pad8(n);
+    void *dst = ws->take(packed_bytes(dtype, rows, dim, n));
+    if (ws->used > ws->cap) return FEQ_ERR_WORKSPACE;
+    const unsigned grid = (unsigned)max64(1, min64((rows * dim * (np / 8) + 255) / 256, (int64_t)sm_count() * 16));
+    uint16_t *d = static_cast<uint16_t *>(dst);
+    if (dtype == FEQ_DTYPE_F32)
+        pack_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float *>(p), rows, dim, n, np, row, comp, d);
+    else
+        pack_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16 *>(p), rows, dim, n, np, row, comp, d);
+    FEQ_LAUNCH_CHECK();
+    o->base = dst;
+    o->comp = np;
+    o->row = (int64_t)dim * np;
+    o->plane = rows * dim * (int64_t)np;
+    o->planes = dtype == FEQ_DTYPE_F32 ? 3 : 1;
+    return FEQ_OK;
+}
+
+template <int MODE, int PLANES, int BN>
+static int launch(const CUtensorMap &am, const CUtensorMap &bm, Params a, const Comps &c, int64_t tiles, cudaStream_t s) {
+    constexpr uint32_t stage = PLANES * (BM + BN) * 128;
+    a.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemLimit - 1024 - kStaging) / stage);
+    const uint32_t smem = 1024 + a.stages * stage + kStaging;
+    auto kern = gemm_kernel<MODE, PLANES, BN>;
+    FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const unsigned grid = (unsigned)max64(1, min64(tiles, sm_count()));
+    kern<<<grid, kThreads, smem, s>>>(am, bm, a, c);
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
+}
+
+// Width of a tile: the widest whose tiles still fill the SMs (a wider tile reads its operands fewer
+// times); float32 keeps three planes of both operands in shared memory, which leaves room for 128.
+static int tile_width(int planes, int64_t row_units, int n) {
+    const int widest = planes == 1 ? 256 : 128;
+    int bn = widest;
+    while (bn > 64 && (n <= bn / 2 || row_units * ((n + bn - 1) / bn) < sm_count())) bn >>= 1;
+    return bn;
+}
+
+template <int MODE>
+static int run(const Operand &A, const Operand &B, Params a, const Comps &c, int bn, int64_t tiles, cudaStream_t s) {
+    CUtensorMap am, bm;
+    int rc = MODE == kGradW ? make_map(&am, A, 1, BK) : make_map(&am, A, 1, BM);
+    if (rc != FEQ_OK) return rc;
+    // weights (matrices, c_out, c_in): the middle dimension is c_out
+    rc = MODE == kGradW ? make_map(&bm, B, 1, BK) : make_map(&bm, B, MODE == kForward ? bn : BK, 1);
+    if (rc != FEQ_OK) return rc;
+    if (A.planes == 3)
+        return bn == 128 ? launch<MODE, 3, 128>(am, bm, a, c, tiles, s) : launch<MODE, 3, 64>(am, bm, a, c, tiles, s);
+    switch (bn) {
+        case 256: return launch<MODE, 1, 256>(am, bm, a, c, tiles, s);
+        case 128: return launch<MODE, 1, 128>(am, bm, a, c, tiles, s);
+        default: return launch<MODE, 1, 64>(am, bm, a, c, tiles, s);
+    }
+}
+
+// kind::f16: D float32, A and B of the same 16-bit type, bits 15 / 16 for MN-major operands.
+static uint32_t instr(int dtype, int bn, bool a_mn, bool b_mn) {
+    const uint32_t f = dtype == FEQ_DTYPE_F16 ? 0u : 1u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
 
 int build_comps(const int32_t *lvals, int32_t n, Comps *c) {
@@ -172,20 +761,34 @@ int build_comps(const int32_t *lvals, int32_t n, Comps *c) {
     for (int i = 0; i < n; i++) {
         if (lvals[i] < 0) return FEQ_ERR_INVALID_ARGUMENT;
         if (lvals[i] > kMaxL || c->dim + 2 * lvals[i] + 1 > kMaxDim) return FEQ_ERR_UNSUPPORTED;
-        for (int m = 0; m < 2 * lvals[i] + 1; m++) {
-            c->rep[c->dim] = (int8_t)i;
-            c->scalar[c->dim++] = (int8_t)(lvals[i] == 0 ? c->scalars : -1);
-        }
-        c->scalars += lvals[i] == 0;
+        c->first[i] = (int16_t)c->dim;
+        c->scalar_of[i] = (int8_t)(lvals[i] == 0 ? c->scalars++ : -1);
+        for (int m = 0; m < 2 * lvals[i] + 1; m++) c->rep[c->dim++] = (int8_t)i;
     }
+    c->first[n] = (int16_t)c->dim;
     return FEQ_OK;
 }
 
-int check(int64_t rows, int32_t experts, int32_t cin, int32_t cout, int32_t dtype) {
-    if (rows < 0 || experts < 1 || cin < 1 || cout < 1 || !dtype_ok(dtype)) return FEQ_ERR_INVALID_ARGUMENT;
-    if (experts > kMaxExperts || rows >= (int64_t)1 << 31) return FEQ_ERR_UNSUPPORTED;
-    return FEQ_OK;
+int check(const FeqExpertLinearArgs &q, Comps *c) {
+    if (q.rows < 0 || q.num_experts < 1 || q.c_in < 1 || q.c_out < 1 || !dtype_ok(q.dtype)) return FEQ_ERR_INVALID_ARGUMENT;
+    if (q.num_experts > kMaxExperts || q.rows >= (int64_t)1 << 31) return FEQ_ERR_UNSUPPORTED;
+    return build_comps(q.lvals, q.n_lvals, c);
 }
+
+// Rows of one part of gW's contraction (0: an expert's rows are one part): the whole expert where its
+// tiles fill the SMs anyway, else enough parts for about two tiles a SM, of 256 rows at least; never more
+// than kLongestPart terms, so that the tensor cores' cut-off stays below 1e-4 of a 16-bit sum.
+int part_rows(const FeqExpertLinearArgs &q, const Comps &c, int bn) {
+    const int64_t base = (int64_t)q.num_experts * c.reps * ((q.c_out + BM - 1) / BM) * ((q.c_in + bn - 1) / bn);
+    const int64_t parts = (2 * 148 + base - 1) / base;
+    int most = 1;
+    for (int i = 0; i < c.reps; i++) most = std::max(most, c.first[i + 1] - c.first[i]);
+    const int64_t longest = kLongestPart / most / 64 * 64;
+    if (parts <= 1) return q.dtype != FEQ_DTYPE_F32 && q.rows > longest ? (int)longest : 0;
+    return (int)min64(longest, max64(256, (q.rows / q.num_experts / parts + 63) / 64 * 64));
+}
+
+int grad_w_width(const FeqExpertLinearArgs &q) { return q.dtype == FEQ_DTYPE_F32 || q.c_in <= 128 ? (q.c_in <= 64 ? 64 : 128) : 256; }
 
 }  // namespace elin
 }  // namespace feq
@@ -195,37 +798,76 @@ using namespace feq::token;
 
 extern "C" size_t feq_expert_linear_workspace_bytes(const FeqExpertLinearArgs *args, int32_t backward) {
     elin::Comps c = {};
-    if (!args || elin::check(args->rows, args->num_experts, args->c_in, args->c_out, args->dtype) != FEQ_OK ||
-        elin::build_comps(args->lvals, args->n_lvals, &c) != FEQ_OK)
-        return 0;
-    return 256;
+    if (!args || elin::check(*args, &c) != FEQ_OK) return 0;
+    const FeqExpertLinearArgs &q = *args;
+    WsCarver ws = {nullptr, 0, 0};
+    ws.take(256);
+    // the operands' packed copies (whether a tensor map serves an operand depends on its address)
+    ws.take(elin::packed_bytes(q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in));
+    ws.take(elin::packed_bytes(q.dtype, q.rows, c.dim, q.c_in));
+    if (backward) {
+        ws.take(elin::packed_bytes(q.dtype, q.rows, c.dim, q.c_out));
+        const int part = elin::part_rows(q, c, elin::grad_w_width(q));
+        if (part > 0)
+            ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
+    }
+    return ws.used;
 }
+
+namespace feq {
+namespace elin {
+
+static Params params(const FeqExpertLinearArgs &q) {
+    Params a = {};
+    a.offsets = q.offsets;
+    a.experts = q.num_experts;
+    a.rows = q.rows;
+    a.out_dtype = a.bias_dtype = q.dtype;
+    a.status = q.status;
+    a.wait_ns = wait_limit_ns();
+    return a;
+}
+
+// y or gx: rows A (rows, dim, K) times the weights.
+template <int MODE>
+static int row_product(const FeqExpertLinearArgs &q, const Comps &c, const Operand &A, const Operand &W, void *out,
+                       cudaStream_t s) {
+    Params a = params(q);
+    a.J = MODE == kForward ? q.c_out : q.c_in;
+    a.K = MODE == kForward ? q.c_in : q.c_out;
+    a.out = out;
+    a.bias = MODE == kForward ? q.bias : nullptr;
+    const int64_t units = ((q.rows + BM - 1) / BM + min64(q.num_experts, q.rows)) * c.dim;
+    const int bn = tile_width(A.planes, (q.rows + BM - 1) / BM * c.dim, a.J);
+    a.idesc = instr(q.dtype, bn, false, MODE == kGradX);
+    return run<MODE>(A, W, a, c, bn, units * ((a.J + bn - 1) / bn), s);
+}
+
+}  // namespace elin
+}  // namespace feq
 
 extern "C" int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *workspace, size_t workspace_bytes,
                                      feq_stream_t stream) {
     if (!args) return FEQ_ERR_INVALID_ARGUMENT;
     const FeqExpertLinearArgs &q = *args;
     elin::Comps c = {};
-    int rc = elin::check(q.rows, q.num_experts, q.c_in, q.c_out, q.dtype);
-    if (rc == FEQ_OK) rc = elin::build_comps(q.lvals, q.n_lvals, &c);
+    int rc = elin::check(q, &c);
     if (rc != FEQ_OK) return rc;
     if (q.rows == 0) return FEQ_OK;
     if (!q.x || !q.weight || !q.offsets || !q.out) return FEQ_ERR_INVALID_ARGUMENT;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+        workspace_bytes < feq_expert_linear_workspace_bytes(args, 0))
+        return FEQ_ERR_WORKSPACE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     ProfScope prof("expert_linear", s);
-    elin::Args a = {};
-    a.w = q.weight;
-    a.rows = q.rows;
-    a.experts = q.num_experts;
-    a.cin = q.c_in;
-    a.cout = q.c_out;
-    a.offsets = q.offsets;
-    const dim3 grid((q.c_out + 63) / 64, (unsigned)((q.rows + 63) / 64 + q.num_experts + 1), c.dim);
-    FEQ_TOKEN_TYPE(q.dtype, elin::rows_kernel<T><<<grid, 256, 0, s>>>(
-                                a, c, static_cast<const T *>(q.x), q.x_row_stride, q.x_comp_stride, q.c_in, q.c_out,
-                                q.c_in, 1, static_cast<const T *>(q.bias), static_cast<T *>(q.out));)
-    FEQ_LAUNCH_CHECK();
-    return FEQ_OK;
+    WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
+    elin::Operand x, w;
+    rc = elin::operand(&x, q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride, &ws, s);
+    if (rc == FEQ_OK)
+        rc = elin::operand(&w, q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in,
+                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s);
+    if (rc != FEQ_OK) return rc;
+    return elin::row_product<elin::kForward>(q, c, x, w, q.out, s);
 }
 
 extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *workspace, size_t workspace_bytes,
@@ -233,43 +875,66 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
     if (!args) return FEQ_ERR_INVALID_ARGUMENT;
     const FeqExpertLinearArgs &q = *args;
     elin::Comps c = {};
-    int rc = elin::check(q.rows, q.num_experts, q.c_in, q.c_out, q.dtype);
-    if (rc == FEQ_OK) rc = elin::build_comps(q.lvals, q.n_lvals, &c);
+    int rc = elin::check(q, &c);
     if (rc != FEQ_OK) return rc;
-    if (!q.offsets || (q.rows && !q.grad_out) || (q.grad_x && !q.weight) || (q.rows && q.grad_weight && !q.x))
-        return FEQ_ERR_INVALID_ARGUMENT;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    const size_t es = dtype_bytes(q.dtype), wsize = (size_t)q.num_experts * c.reps * q.c_in * q.c_out;
+    if (q.rows == 0) {                      // empty sums
+        if (q.grad_weight) FEQ_CUDA_TRY(cudaMemsetAsync(q.grad_weight, 0, wsize * es, s));
+        if (q.grad_bias) FEQ_CUDA_TRY(cudaMemsetAsync(q.grad_bias, 0, (size_t)q.num_experts * c.scalars * q.c_out * es, s));
+        return FEQ_OK;
+    }
+    if (!q.offsets || !q.grad_out || (q.grad_x && !q.weight) || (q.grad_weight && !q.x)) return FEQ_ERR_INVALID_ARGUMENT;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+        workspace_bytes < feq_expert_linear_workspace_bytes(args, 1))
+        return FEQ_ERR_WORKSPACE;
     ProfScope prof("expert_linear_bwd", s);
-    elin::Args a = {};
-    a.x = q.x;
-    a.w = q.weight;
-    a.gy = q.grad_out;
-    a.gw = q.grad_weight;
-    a.gb = q.grad_bias;
-    a.rows = q.rows;
-    a.x_row = q.x_row_stride;
-    a.x_comp = q.x_comp_stride;
-    a.gy_row = q.grad_row_stride;
-    a.gy_comp = q.grad_comp_stride;
-    a.experts = q.num_experts;
-    a.cin = q.c_in;
-    a.cout = q.c_out;
-    a.offsets = q.offsets;
-    if (q.grad_x && q.rows) {
-        const dim3 grid((q.c_in + 63) / 64, (unsigned)((q.rows + 63) / 64 + q.num_experts + 1), c.dim);
-        FEQ_TOKEN_TYPE(q.dtype, elin::rows_kernel<T><<<grid, 256, 0, s>>>(
-                                    a, c, static_cast<const T *>(q.grad_out), q.grad_row_stride, q.grad_comp_stride,
-                                    q.c_out, q.c_in, 1, q.c_in, nullptr, static_cast<T *>(q.grad_x));)
-        FEQ_LAUNCH_CHECK();
+    WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
+    elin::Operand g, x, w;
+    if (q.grad_x || q.grad_weight) {
+        rc = elin::operand(&g, q.grad_out, q.dtype, q.rows, c.dim, q.c_out, q.grad_row_stride, q.grad_comp_stride, &ws, s);
+        if (rc != FEQ_OK) return rc;
+    }
+    if (q.grad_x) {
+        rc = elin::operand(&w, q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in,
+                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s);
+        if (rc == FEQ_OK) rc = elin::row_product<elin::kGradX>(q, c, g, w, q.grad_x, s);
+        if (rc != FEQ_OK) return rc;
     }
     if (q.grad_weight) {
-        const dim3 grid((q.c_in + 63) / 64, (q.c_out + 63) / 64, q.num_experts * c.reps);
-        FEQ_TOKEN_TYPE(q.dtype, elin::weights_kernel<T><<<grid, 256, 0, s>>>(a, c);)
-        FEQ_LAUNCH_CHECK();
+        rc = elin::operand(&x, q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride, &ws, s);
+        if (rc != FEQ_OK) return rc;
+        const int bn = elin::grad_w_width(q), part = elin::part_rows(q, c, bn);
+        elin::Params a = elin::params(q);
+        a.J = q.c_out;
+        a.K = q.c_in;
+        a.split = part > 0;
+        a.chunk_rows = part > 0 ? part : (int)((q.rows + 63) / 64 * 64);
+        const int64_t parts = part > 0 ? q.rows / part + q.num_experts : q.num_experts;
+        a.out = q.grad_weight;
+        if (a.split) {
+            a.out = ws.take((size_t)parts * c.reps * q.c_in * q.c_out * sizeof(float));
+            if (ws.used > ws.cap) return FEQ_ERR_WORKSPACE;
+            a.out_dtype = FEQ_DTYPE_F32;
+        }
+        a.idesc = elin::instr(q.dtype, bn, true, true);
+        const int64_t tiles = parts * c.reps * ((q.c_out + elin::BM - 1) / elin::BM) * ((q.c_in + bn - 1) / bn);
+        rc = elin::run<elin::kGradW>(g, x, a, c, bn, tiles, s);
+        if (rc != FEQ_OK) return rc;
+        if (a.split) {
+            const int64_t size = (int64_t)q.c_in * q.c_out;
+            const dim3 grid((unsigned)min64((size + 255) / 256, 64), (unsigned)(q.num_experts * c.reps));
+            FEQ_TOKEN_TYPE(q.dtype, elin::join_kernel<T><<<grid, 256, 0, s>>>(
+                                        static_cast<const float *>(a.out), q.offsets, q.num_experts, q.rows, part, c.reps,
+                                        size, static_cast<T *>(q.grad_weight));)
+            FEQ_LAUNCH_CHECK();
+        }
     }
     if (q.grad_bias && c.scalars) {
         const dim3 grid((q.c_out + 31) / 32, q.num_experts * c.scalars);
-        FEQ_TOKEN_TYPE(q.dtype, elin::bias_kernel<T><<<grid, 1024, 0, s>>>(a, c);)
+        FEQ_TOKEN_TYPE(q.dtype, elin::bias_kernel<T><<<grid, 1024, 0, s>>>(
+                                    static_cast<const T *>(q.grad_out), q.grad_row_stride, q.grad_comp_stride, q.offsets,
+                                    q.num_experts, q.rows, q.c_out, c, static_cast<T *>(q.grad_bias));)
         FEQ_LAUNCH_CHECK();
     }
     return FEQ_OK;
