@@ -796,22 +796,39 @@ int grad_w_width(const FeqExpertLinearArgs &q) { return q.dtype == FEQ_DTYPE_F32
 using namespace feq;
 using namespace feq::token;
 
+namespace feq {
+namespace elin {
+
+// Bytes of workspace that the call needs: the packed copies of operands that no tensor map
+// describes as they lie, and gW's partial sums.
+static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool backward) {
+    WsCarver ws = {nullptr, 0, 0};
+    auto pack = [&](const void *p, int64_t rows, int dim, int n, int64_t row, int64_t comp) {
+        if (!mappable(p, q.dtype, rows, dim, n, row, comp)) ws.take(packed_bytes(q.dtype, rows, dim, n));
+    };
+    const int64_t matrices = (int64_t)q.num_experts * c.reps;
+    if (backward && (q.grad_x || q.grad_weight))
+        pack(q.grad_out, q.rows, c.dim, q.c_out, q.grad_row_stride, q.grad_comp_stride);
+    if (!backward || q.grad_x) pack(q.weight, matrices, q.c_out, q.c_in, (int64_t)q.c_out * q.c_in, q.c_in);
+    if (!backward || q.grad_weight) pack(q.x, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride);
+    if (backward && q.grad_weight) {
+        const int part = part_rows(q, c, grad_w_width(q));
+        if (part > 0) ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
+    }
+    return (ws.used + 255) & ~size_t(255);       // in any order of the regions
+}
+
+static bool workspace_ok(const void *p, size_t bytes, size_t need) {
+    return need == 0 || (p && !(reinterpret_cast<uintptr_t>(p) & 15) && bytes >= need);
+}
+
+}  // namespace elin
+}  // namespace feq
+
 extern "C" size_t feq_expert_linear_workspace_bytes(const FeqExpertLinearArgs *args, int32_t backward) {
     elin::Comps c = {};
     if (!args || elin::check(*args, &c) != FEQ_OK) return 0;
-    const FeqExpertLinearArgs &q = *args;
-    WsCarver ws = {nullptr, 0, 0};
-    ws.take(256);
-    // the operands' packed copies (whether a tensor map serves an operand depends on its address)
-    ws.take(elin::packed_bytes(q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in));
-    ws.take(elin::packed_bytes(q.dtype, q.rows, c.dim, q.c_in));
-    if (backward) {
-        ws.take(elin::packed_bytes(q.dtype, q.rows, c.dim, q.c_out));
-        const int part = elin::part_rows(q, c, elin::grad_w_width(q));
-        if (part > 0)
-            ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
-    }
-    return ws.used;
+    return std::max<size_t>(256, elin::workspace_need(*args, c, backward != 0));
 }
 
 namespace feq {
@@ -855,9 +872,7 @@ extern "C" int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *work
     if (rc != FEQ_OK) return rc;
     if (q.rows == 0) return FEQ_OK;
     if (!q.x || !q.weight || !q.offsets || !q.out) return FEQ_ERR_INVALID_ARGUMENT;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-        workspace_bytes < feq_expert_linear_workspace_bytes(args, 0))
-        return FEQ_ERR_WORKSPACE;
+    if (!elin::workspace_ok(workspace, workspace_bytes, elin::workspace_need(q, c, false))) return FEQ_ERR_WORKSPACE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     ProfScope prof("expert_linear", s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
@@ -885,9 +900,7 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
         return FEQ_OK;
     }
     if (!q.offsets || !q.grad_out || (q.grad_x && !q.weight) || (q.grad_weight && !q.x)) return FEQ_ERR_INVALID_ARGUMENT;
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
-        workspace_bytes < feq_expert_linear_workspace_bytes(args, 1))
-        return FEQ_ERR_WORKSPACE;
+    if (!elin::workspace_ok(workspace, workspace_bytes, elin::workspace_need(q, c, true))) return FEQ_ERR_WORKSPACE;
     ProfScope prof("expert_linear_bwd", s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
     elin::Operand g, x, w;

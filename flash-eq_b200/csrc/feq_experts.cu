@@ -26,11 +26,10 @@ namespace experts {
 using namespace token;
 
 constexpr int kMaxExperts = 512, kMaxTopK = 32;
-constexpr int kPerLane = kMaxExperts / 32;
 constexpr int kSmallPairs = 4096;             // one block routes these
 constexpr int kSmallThreads = 1024;
 constexpr int kPlaceThreads = 256;
-constexpr int kPlacePairs = 2048;             // pairs of one placing block
+constexpr int kPlacePairs = 4096;             // pairs of one placing block, at most
 
 struct Route {
     const void *logits;
@@ -51,19 +50,21 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One warp chooses the experts of one token; lane j < top_k ends up with choice j (id -1: none).
-template <typename T>
+// One warp chooses the experts of one token, L logits a lane; lane j < top_k ends up with choice j
+// (id -1: none).
+template <typename T, int L>
 __device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, float &my_w) {
     const int lane = threadIdx.x & 31;
     const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-    float v[kPerLane];
-    uint32_t key[kPerLane];
-    uint32_t top = 0;
+    float v[L];
+    uint32_t key[L], top = 0;
 #pragma unroll
-    for (int i = 0; i < kPerLane; i++) {
+    for (int i = 0; i < L; i++) {
         const int e = i * 32 + lane;
-        if (i * 32 >= a.experts) break;
         v[i] = e < a.experts ? to_f32(row[e]) : -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < L; i++) {
         key[i] = rank_key(v[i]);
         top = max(top, key[i]);
     }
@@ -75,8 +76,7 @@ __device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, fl
         int e = 0x7fffffff;
         float val = 0.0f;
 #pragma unroll
-        for (int i = kPerLane - 1; i >= 0; i--) {
-            if (i * 32 >= a.experts) continue;
+        for (int i = L - 1; i >= 0; i--) {
             if (key[i] == best) {
                 e = i * 32 + lane;
                 val = v[i];
@@ -91,8 +91,7 @@ __device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, fl
         }
         top = 0;
 #pragma unroll
-        for (int i = 0; i < kPerLane; i++) {
-            if (i * 32 >= a.experts) break;
+        for (int i = 0; i < L; i++) {
             if (i * 32 + lane == win) key[i] = 0u;
             top = max(top, key[i]);
         }
@@ -104,14 +103,19 @@ __device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, fl
     } else {
         float s = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kPerLane; i++) {
-            if (i * 32 >= a.experts) break;
-            s += expf(v[i] - biggest);
-        }
+        for (int i = 0; i < L; i++) s += expf(v[i] - biggest);
         total = lane_sum(s, 32);
     }
     if (my_id >= 0) my_w /= total;
 }
+
+// Calls f with the number of logits a lane as a constant.
+#define FEQ_EXPERTS_PER_LANE(experts, ...)                                                \
+    if ((experts) <= 32) { constexpr int L = 1; __VA_ARGS__ }                             \
+    else if ((experts) <= 64) { constexpr int L = 2; __VA_ARGS__ }                        \
+    else if ((experts) <= 128) { constexpr int L = 4; __VA_ARGS__ }                       \
+    else if ((experts) <= 256) { constexpr int L = 8; __VA_ARGS__ }                       \
+    else { constexpr int L = 16; __VA_ARGS__ }
 
 // Counts of the pairs [lo, hi) of `key` (experts for none) per expert, one warp, into hist.
 __device__ __forceinline__ void warp_count(const int16_t *key, int lo, int hi, int32_t *hist) {
@@ -173,7 +177,7 @@ __device__ __forceinline__ void warp_starts(int32_t *hist, int warps, int n, int
 }
 
 // The whole routing of up to kSmallPairs pairs in one block.
-template <typename T>
+template <typename T, int L>
 __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const Route a) {
     extern __shared__ int32_t sh[];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const Route 
     for (int n = warp; n < (int)a.tokens; n += warps) {
         int id;
         float w;
-        choose<T>(a, n, id, w);
+        choose<T, L>(a, n, id, w);
         if (lane < a.top_k) {
             const int p = n * a.top_k + lane;
             a.ids[p] = id;
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const Route 
 }
 
 // Step 1 of 3: choose, and count a block's pairs per expert.
-template <typename T>
+template <typename T, int L>
 __global__ void __launch_bounds__(kPlaceThreads) route_choose_kernel(const Route a) {
     extern __shared__ int32_t sh[];
     const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(kPlaceThreads) route_choose_kernel(const Route
     for (int64_t n = n0 + warp; n < n1; n += warps) {
         int id;
         float w;
-        choose<T>(a, n, id, w);
+        choose<T, L>(a, n, id, w);
         if (lane < a.top_k) {
             const int64_t p = n * a.top_k + lane;
             a.ids[p] = id;
@@ -442,8 +446,11 @@ __global__ void __launch_bounds__(256) combine_bwd_kernel(const Rows a) {
     }
 }
 
+// Blocks of choosing and placing: of 256 pairs (8 warps choose a few tokens each, one after the other)
+// up to a million pairs, then larger, which keeps the table of counts small.
 int route_plan(int64_t tokens, int top_k, int *per) {
-    const int t = kPlacePairs / top_k;
+    const int64_t pairs = min64(kPlacePairs, max64(256, tokens * top_k / 4096));
+    const int t = (int)max64(1, pairs / top_k);
     *per = t;
     return (int)((tokens + t - 1) / t);
 }
@@ -463,7 +470,7 @@ using namespace feq;
 using namespace feq::token;
 
 extern "C" size_t feq_expert_route_workspace_bytes(int64_t tokens, int32_t top_k, int32_t experts) {
-    if (experts::check(tokens, top_k, experts) != FEQ_OK) return 0;
+    if (experts::check(tokens, top_k, experts) != FEQ_OK || tokens * top_k <= experts::kSmallPairs) return 0;
     int per;
     const int blocks = experts::route_plan(tokens, top_k, &per);
     return (size_t)(experts + 1) * ((size_t)blocks + 1) * sizeof(int32_t);
@@ -497,12 +504,12 @@ extern "C" int feq_expert_route(const void *logits, int64_t tokens, int64_t stri
     if (tokens * top_k <= experts::kSmallPairs) {
         const int warps = (int)min64(experts::kSmallThreads / 32, max64(tokens, 1));
         const size_t smem = (size_t)(warps + 2) * nk * 4 + (size_t)tokens * top_k * 2;
-        FEQ_TOKEN_TYPE(dtype, {
-            auto kern = experts::route_small_kernel<T>;
+        FEQ_TOKEN_TYPE(dtype, FEQ_EXPERTS_PER_LANE(num_experts, {
+            auto kern = experts::route_small_kernel<T, L>;
             if (smem > 48 * 1024)
                 FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             kern<<<1, warps * 32, smem, s>>>(a);
-        })
+        }))
         FEQ_LAUNCH_CHECK();
         return FEQ_OK;
     }
@@ -512,7 +519,9 @@ extern "C" int feq_expert_route(const void *logits, int64_t tokens, int64_t stri
     a.counts = static_cast<int32_t *>(workspace);
     int32_t *totals = a.counts + (size_t)nk * a.blocks;
     const size_t smem = (size_t)(experts::kPlaceThreads / 32 + 2) * nk * 4 + experts::kPlacePairs * 2;
-    FEQ_TOKEN_TYPE(dtype, experts::route_choose_kernel<T><<<a.blocks, experts::kPlaceThreads, nk * 4, s>>>(a);)
+    FEQ_TOKEN_TYPE(dtype, FEQ_EXPERTS_PER_LANE(num_experts, {
+        experts::route_choose_kernel<T, L><<<a.blocks, experts::kPlaceThreads, nk * 4, s>>>(a);
+    }))
     FEQ_LAUNCH_CHECK();
     experts::route_prefix_kernel<<<nk, 256, 0, s>>>(a, totals);
     FEQ_LAUNCH_CHECK();

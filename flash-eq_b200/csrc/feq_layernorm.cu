@@ -10,11 +10,15 @@
 // the centred sum of squares are exact two-pass sums over registers and the row is read once.
 // A thread owns the same columns for every row of its group, so w and b are read once per
 // thread and, backwards, gw and gb are summed in registers over the group's rows; the groups of
-// a block join in shared memory and the blocks in a second kernel, all in a fixed order.
+// a block join in shared memory and the blocks in a second kernel, all in a fixed order.  The next
+// rows are copied to shared memory while the current one is summed.  Rows of odd widths are read in 16-byte vectors that
+// straddle their ends (row_shift).
 // Products that enter the row's sums, and u mean(g w u), are rounded before they are added: in rows of
 // two the terms of gx cancel down to eps / v of their size, and a product kept longer on one side only
 // would be what is left.
 // Rows wider than kMaxWidth go through kernels that stream the row from L2 instead.
+#include <algorithm>
+
 #include "feq_token.cuh"
 
 namespace feq {
@@ -24,7 +28,7 @@ using namespace token;
 
 constexpr int kBlock = 256;
 constexpr int kMaxTpr = 512;
-constexpr int kMaxWidth = 16 * kMaxTpr;      // 16 elements a thread
+constexpr int kMaxWidth = 16 * kMaxTpr - 8;  // 16 elements a thread, the first up to 7 before the row
 constexpr int kLimitWidth = 1 << 29;         // column arithmetic stays in 32 bits
 constexpr int kReduceCols = 32;
 
@@ -38,149 +42,299 @@ struct Args {
     float eps;
 };
 
-// Sum over the `tpr` threads of a group.  tpr > 32: red holds one value per warp of the block and
-// each group has a named barrier; `slot` alternates so that one barrier per sum is enough.
-__device__ __forceinline__ float group_sum(float v, int tpr, float (*red)[32], int &slot) {
-    if (tpr <= 32) return lane_sum(v, tpr);
-    v = lane_sum(v, 32);
-    const int nw = tpr >> 5, lane = threadIdx.x & 31, group = threadIdx.x / tpr;
-    if (lane == 0) red[slot][threadIdx.x >> 5] = v;
-    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
-    const float s = lane < nw ? red[slot][group * nw + lane] : 0.0f;
-    slot ^= 1;
-    return lane_sum(s, 32);
-}
-
-// Element e of a thread's row part is column (e / V * tpr + t) * V + e % V.
-template <typename T, int V, int E>
-__device__ __forceinline__ void load_row(const T *row, int width, int tpr, int t, float (&v)[E]) {
-    constexpr int N = E / V;
-    Pack<T, V> p[N];
+// Sums of K values over the `tpr` threads of a group, the same in every thread.  tpr > 32: red holds K
+// values per warp of the block and each group has a named barrier; `slot` alternates so that one
+// barrier per call is enough.
+template <int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float (*red)[K][16], int &slot) {
+    if (tpr < 32) {
+        for (int o = tpr >> 1; o > 0; o >>= 1) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int c = (i * tpr + t) * V;
-        if (c < width) p[i] = *reinterpret_cast<const Pack<T, V> *>(row + c);
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int c = (i * tpr + t) * V;
-#pragma unroll
-        for (int q = 0; q < V; q++) v[i * V + q] = c < width ? to_f32(p[i].v[q]) : 0.0f;
-    }
-}
-
-template <typename T, int V, int E>
-__device__ __forceinline__ void store_row(T *row, int width, int tpr, int t, const float (&v)[E]) {
-#pragma unroll
-    for (int i = 0; i < E / V; i++) {
-        const int c = (i * tpr + t) * V;
-        if (c < width) {
-            Pack<T, V> p;
-#pragma unroll
-            for (int q = 0; q < V; q++) p.v[q] = from_f32<T>(v[i * V + q]);
-            *reinterpret_cast<Pack<T, V> *>(row + c) = p;
+            for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
         }
+        return;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    }
+    if (tpr == 32) return;
+    const int nw = tpr >> 5, group = threadIdx.x / tpr;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int k = 0; k < K; k++) red[slot][k][threadIdx.x >> 5] = v[k];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(tpr) : "memory");
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const float *p = &red[slot][k][group * nw];
+        float s;
+        if (nw == 2) {
+            const float2 f = *reinterpret_cast<const float2 *>(p);
+            s = f.x + f.y;
+        } else {
+            s = 0.0f;
+            for (int i = 0; i < nw; i += 4) {
+                const float4 f = *reinterpret_cast<const float4 *>(p + i);
+                s += (f.x + f.y) + (f.z + f.w);
+            }
+        }
+        v[k] = s;
+    }
+    slot ^= 1;
 }
 
-template <typename T, int V, int E>
-__device__ __forceinline__ void load_param(const void *p, int is_f32, float otherwise, int width, int tpr, int t,
-                                           float (&v)[E]) {
+// A thread's part of a row: N = E / V vectors, vector i covers the columns from (i * tpr + t) * V - shift on.
+// shift (kShift) is how far the row starts behind a 16-byte boundary, in elements: the vectors lie on
+// the boundary whatever the row's address, and the first and the last are moved by elements.
+template <int V>
+__device__ __forceinline__ int column(int e, int tpr, int t, int shift) { return (e / V * tpr + t) * V - shift + e % V; }
+
+// Bit e: element e of the thread is a column of the row.
+template <int V, int E>
+__device__ __forceinline__ uint32_t columns_of(int width, int tpr, int t, int shift) {
+    uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const int c = (e / V * tpr + t) * V + e % V;
-        v[e] = p && c < width ? param_at<T>(p, is_f32, c) : otherwise;
+        const int c = column<V>(e, tpr, t, shift);
+        if (c >= 0 && c < width) m |= 1u << e;
+    }
+    return m;
+}
+
+// Rows in flight.  16-byte vectors go through a ring in shared memory that each thread fills (cp.async)
+// and reads for itself, kAhead rows ahead, so that what is in flight takes no registers and needs no
+// barrier; narrower ones are loaded when they are used.
+constexpr int kStages = 3, kAhead = kStages - 1;
+
+template <typename T, int V, int E, bool kShift>
+struct Stream {
+    static constexpr bool kRing = V * sizeof(T) == 16;
+    static constexpr int N = E / V;
+    uint8_t *ring;                            // kStages slots, `slot_bytes` apart
+    uint32_t slot_bytes;
+    const T *base;
+    int64_t stride, rows;
+    int width, tpr, t, shift;
+
+    __device__ __forceinline__ const T *row(int64_t r) const { return base + r * stride; }
+    __device__ __forceinline__ Pack<T, V> *slot(int s, int i) const {
+        return reinterpret_cast<Pack<T, V> *>(ring + s * slot_bytes + (i * blockDim.x + threadIdx.x) * 16);
+    }
+    __device__ __forceinline__ Pack<T, V> edge(const T *p, int c) const {      // some elements lie outside the row
+        Pack<T, V> d;
+#pragma unroll
+        for (int q = 0; q < V; q++) d.v[q] = c + q >= 0 && c + q < width ? p[c + q] : from_f32<T>(0.0f);
+        return d;
+    }
+    __device__ __forceinline__ void fetch(int64_t r, int s) const {
+        if (!kRing || r >= rows) return;
+        const T *p = row(r);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = (i * tpr + t) * V - (kShift ? shift : 0);
+            if (kShift ? c >= 0 && c + V <= width : c < width)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                 static_cast<uint32_t>(__cvta_generic_to_shared(slot(s, i)))), "l"(p + c) : "memory");
+            else if (kShift && c + V > 0 && c < width)
+                *slot(s, i) = edge(p, c);
+        }
+    }
+    // zeros where the thread has no column
+    __device__ __forceinline__ void read(int64_t r, int s, float (&v)[E]) const {
+        Pack<T, V> d[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = (i * tpr + t) * V - (kShift ? shift : 0);
+            if (r < rows && (kShift ? c + V > 0 && c < width : c < width)) {
+                if (kRing) d[i] = *slot(s, i);
+                else d[i] = *reinterpret_cast<const Pack<T, V> *>(row(r) + c);
+            } else {
+#pragma unroll
+                for (int q = 0; q < V; q++) d[i].v[q] = from_f32<T>(0.0f);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = to_f32(d[e / V].v[e % V]);
+    }
+};
+
+__device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wait_row() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+
+template <typename T, int V, int E, bool kShift>
+__device__ __forceinline__ void store_part(T *row, int width, int tpr, int t, int shift, const float (&v)[E]) {
+#pragma unroll
+    for (int i = 0; i < E / V; i++) {
+        const int c = (i * tpr + t) * V - (kShift ? shift : 0);
+        Pack<T, V> p;
+#pragma unroll
+        for (int q = 0; q < V; q++) p.v[q] = from_f32<T>(v[i * V + q]);
+        if (kShift ? c >= 0 && c + V <= width : c < width) {
+            *reinterpret_cast<Pack<T, V> *>(row + c) = p;
+        } else if (kShift) {
+#pragma unroll
+            for (int q = 0; q < V; q++)
+                if (c + q >= 0 && c + q < width) row[c + q] = p.v[q];
+        }
     }
 }
 
 template <typename T, int V, int E>
-__global__ void __launch_bounds__(kMaxTpr) forward_kernel(const Args a) {
-    __shared__ float red[2][32];
-    int slot = 0;
-    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
-    const int groups = blockDim.x / tpr;
-    float w[E], b[E];
-    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, w);
-    load_param<T, V, E>(a.b, a.param_f32, 0.0f, a.width, tpr, t, b);
-    const float inv = 1.0f / (float)a.width;
-    // every thread of a warp makes the same number of rounds: the sums are warp-wide
-    const int64_t step = (int64_t)gridDim.x * groups;
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
-        const int64_t r = r0 + threadIdx.x / tpr;
-        const bool live = r < a.rows;
-        const int width = live ? a.width : 0;
-        float x[E];
-        load_row<T, V, E>(static_cast<const T *>(a.x) + (live ? r * a.x_stride : 0), width, tpr, t, x);
-        float s = 0.0f;
+__device__ __forceinline__ void load_param(const void *p, int is_f32, float otherwise, int width, int tpr, int t, int shift,
+                                           float (&v)[E]) {
 #pragma unroll
-        for (int e = 0; e < E; e++) s += x[e];
-        const float mu = group_sum(s, tpr, red, slot) * inv;
-        float q = 0.0f;
+    for (int e = 0; e < E; e++) v[e] = otherwise;
+    if (!p) return;
+    if (is_f32) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int c = (e / V * tpr + t) * V;
-            const float d = c < width ? x[e] - mu : 0.0f;
-            x[e] = d;
-            q += __fmul_rn(d, d);
+            const int c = column<V>(e, tpr, t, shift);
+            if (c >= 0 && c < width) v[e] = static_cast<const float *>(p)[c];
         }
-        const float rstd = rsqrtf(group_sum(q, tpr, red, slot) * inv + a.eps);
-        if (live && t == 0 && a.mean) {
-            a.mean[r] = mu;
-            a.rstd[r] = rstd;
-        }
+    } else {
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = x[e] * rstd * w[e] + b[e];
-        store_row<T, V, E>(static_cast<T *>(a.y) + (live ? r * (int64_t)a.width : 0), width, tpr, t, x);
+        for (int e = 0; e < E; e++) {
+            const int c = column<V>(e, tpr, t, shift);
+            if (c >= 0 && c < width) v[e] = to_f32(static_cast<const T *>(p)[c]);
+        }
     }
 }
 
-template <typename T, int V, int E>
-__global__ void __launch_bounds__(kMaxTpr) backward_kernel(const Args a) {
-    __shared__ float red[2][32];
-    extern __shared__ float sums[];           // (2, width): gw and gb of this block
+// Elements between the 16-byte boundary below a row's address and the row.  The same for every row
+// of a group: the rows of a group lie a multiple of V rows apart.
+template <typename T, int V, bool kShift>
+__device__ __forceinline__ int row_shift(const void *base, int64_t row, int64_t stride) {
+    if (!kShift) return 0;
+    return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(row * stride)) & (V - 1));
+}
+
+template <typename T, int V, int E, bool kShift>
+__global__ void __launch_bounds__(kMaxTpr) forward_kernel(const Args a) {
+    __shared__ __align__(16) float red[2][1][16];
+    extern __shared__ __align__(16) uint8_t ring[];
     int slot = 0;
-    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr;
-    const int groups = blockDim.x / tpr;
+    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x / tpr;
+    const int64_t first = (int64_t)blockIdx.x * groups + threadIdx.x / tpr, step = (int64_t)gridDim.x * groups;
+    const int shift = row_shift<T, V, kShift>(a.x, first, a.x_stride);
+    const Stream<T, V, E, kShift> x = {ring, (uint32_t)(E / V * blockDim.x * 16), static_cast<const T *>(a.x), a.x_stride,
+                                       a.rows, a.width, tpr, t, shift};
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+        x.fetch(first + k * step, k);
+        fetched();
+    }
+    float w[E], b[E];
+    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, shift, w);
+    load_param<T, V, E>(a.b, a.param_f32, 0.0f, a.width, tpr, t, shift, b);
+    const uint32_t mine = columns_of<V, E>(a.width, tpr, t, shift);
+    const float inv = 1.0f / (float)a.width;
+    // every thread of a warp makes the same number of rounds: the sums are warp-wide
+    const int64_t rounds = (a.rows - (int64_t)blockIdx.x * groups + step - 1) / step;
+    int64_t r = first;
+    for (int64_t i = 0; i < rounds; i++, r += step) {
+        const int s = (int)(i % kStages);
+        wait_row();
+        float v[E];
+        x.read(r, s, v);
+        x.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
+        fetched();
+        float m[1] = {0.0f}, q[1] = {0.0f};
+#pragma unroll
+        for (int e = 0; e < E; e++) m[0] += v[e];
+        group_sum<1>(m, tpr, red, slot);
+        const float mu = m[0] * inv;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            v[e] = mine & (1u << (kShift ? e : e / V * V)) ? v[e] - mu : 0.0f;
+            q[0] += __fmul_rn(v[e], v[e]);
+        }
+        group_sum<1>(q, tpr, red, slot);
+        const float rstd = rsqrtf(q[0] * inv + a.eps);
+        if (r < a.rows) {
+            if (t == 0 && a.mean) {
+                a.mean[r] = mu;
+                a.rstd[r] = rstd;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = v[e] * rstd * w[e] + b[e];
+            store_part<T, V, E, kShift>(static_cast<T *>(a.y) + r * (int64_t)a.width, a.width, tpr, t, shift, v);
+        }
+    }
+}
+
+template <typename T, int V, int E, bool kShift>
+__global__ void __launch_bounds__(kMaxTpr) backward_kernel(const Args a) {
+    __shared__ __align__(16) float red[2][2][16];
+    extern __shared__ __align__(16) uint8_t ring[];      // the rings of x and g; at the end (2, width) sums
+    int slot = 0;
+    const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
+    const int64_t first = (int64_t)blockIdx.x * groups + group, step = (int64_t)gridDim.x * groups;
+    const int shift = row_shift<T, V, kShift>(a.x, first, a.x_stride);
+    const uint32_t part = E / V * blockDim.x * 16;
+    const Stream<T, V, E, kShift> x = {ring, 2 * part, static_cast<const T *>(a.x), a.x_stride, a.rows, a.width, tpr, t, shift};
+    const Stream<T, V, E, kShift> g = {ring + part, 2 * part, static_cast<const T *>(a.g), a.g_stride, a.rows, a.width, tpr, t, shift};
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+        x.fetch(first + k * step, k);
+        g.fetch(first + k * step, k);
+        fetched();
+    }
     float w[E], gw[E], gb[E];
-    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, w);
+    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, shift, w);
+    const uint32_t mine = columns_of<V, E>(a.width, tpr, t, shift);
 #pragma unroll
     for (int e = 0; e < E; e++) gw[e] = gb[e] = 0.0f;
     const float inv = 1.0f / (float)a.width;
-    const int64_t step = (int64_t)gridDim.x * groups;
-    for (int64_t r0 = (int64_t)blockIdx.x * groups; r0 < a.rows; r0 += step) {
-        const int64_t r = r0 + group;
-        const bool live = r < a.rows;
-        const int width = live ? a.width : 0;
-        float x[E], g[E];
-        load_row<T, V, E>(static_cast<const T *>(a.x) + (live ? r * a.x_stride : 0), width, tpr, t, x);
-        load_row<T, V, E>(static_cast<const T *>(a.g) + (live ? r * a.g_stride : 0), width, tpr, t, g);
-        const float mu = live ? a.mean[r] : 0.0f, rstd = live ? a.rstd[r] : 0.0f;
-        float s1 = 0.0f, s2 = 0.0f;
+    const int64_t rounds = (a.rows - (int64_t)blockIdx.x * groups + step - 1) / step;
+    int64_t r = first;
+    float mu_n = r < a.rows ? a.mean[r] : 0.0f, rstd_n = r < a.rows ? a.rstd[r] : 0.0f;
+    for (int64_t i = 0; i < rounds; i++, r += step) {
+        const int s = (int)(i % kStages);
+        const float mu = mu_n, rstd = rstd_n;
+        if (r + step < a.rows) {
+            mu_n = a.mean[r + step];
+            rstd_n = a.rstd[r + step];
+        }
+        wait_row();
+        float u[E], v[E];
+        x.read(r, s, u);
+        g.read(r, s, v);
+        x.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
+        g.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
+        fetched();
+        float m[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            const int c = (e / V * tpr + t) * V;
-            const float u = c < width ? (x[e] - mu) * rstd : 0.0f;
-            gw[e] += g[e] * u;
-            gb[e] += g[e];
-            x[e] = u;
-            g[e] *= w[e];
-            s1 += g[e];
-            s2 += __fmul_rn(g[e], u);
+            u[e] = mine & (1u << (kShift ? e : e / V * V)) ? (u[e] - mu) * rstd : 0.0f;
+            gw[e] += v[e] * u[e];
+            gb[e] += v[e];
+            v[e] *= w[e];
+            m[0] += v[e];
+            m[1] += __fmul_rn(v[e], u[e]);
         }
-        s1 = group_sum(s1, tpr, red, slot) * inv;
-        s2 = group_sum(s2, tpr, red, slot) * inv;
+        if (!a.gx) continue;
+        group_sum<2>(m, tpr, red, slot);
+        const float s1 = m[0] * inv, s2 = m[1] * inv;
+        if (r < a.rows) {
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = rstd * (g[e] - s1 - __fmul_rn(x[e], s2));
-        if (a.gx) store_row<T, V, E>(static_cast<T *>(a.gx) + (live ? r * (int64_t)a.width : 0), width, tpr, t, x);
+            for (int e = 0; e < E; e++) u[e] = rstd * (v[e] - s1 - __fmul_rn(u[e], s2));
+            store_part<T, V, E, kShift>(static_cast<T *>(a.gx) + r * (int64_t)a.width, a.width, tpr, t, shift, u);
+        }
     }
     if (!a.partial) return;
-    // join the groups in their order
+    // join the groups in their order; rows past the end added nothing (mu, rstd of a finished group are stale,
+    // its g is zero)
+    float *sums = reinterpret_cast<float *>(ring);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
     for (int k = 0; k < groups; k++) {
         if (group == k) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const int c = (e / V * tpr + t) * V + e % V;
-                if (c < a.width) {
+                const int c = column<V>(e, tpr, t, shift);
+                if (c >= 0 && c < a.width) {
                     sums[c] = (k ? sums[c] : 0.0f) + gw[e];
                     sums[a.width + c] = (k ? sums[a.width + c] : 0.0f) + gb[e];
                 }
@@ -216,7 +370,16 @@ reduce_kernel(const float *__restrict__ partial, int blocks, int width, int para
     }
 }
 
-// ---- rows wider than kMaxWidth: one block a row, the row streamed once per sum ----
+// ---- rows wider than kMaxWidth: one block of 1024 a row, the row streamed once per sum ----
+__device__ __forceinline__ float block_sum(float v, float (*red)[32], int &slot) {
+    v = lane_sum(v, 32);
+    if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane_sum(red[slot][threadIdx.x & 31], 32);
+    slot ^= 1;
+    return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024) wide_forward_kernel(const Args a) {
     __shared__ float red[2][32];
@@ -227,12 +390,12 @@ __global__ void __launch_bounds__(1024) wide_forward_kernel(const Args a) {
         T *y = static_cast<T *>(a.y) + r * (int64_t)a.width;
         float s = 0.0f, q = 0.0f;
         for (int c = threadIdx.x; c < a.width; c += blockDim.x) s += to_f32(x[c]);
-        const float mu = group_sum(s, blockDim.x, red, slot) * inv;
+        const float mu = block_sum(s, red, slot) * inv;
         for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
             const float d = to_f32(x[c]) - mu;
             q += d * d;
         }
-        const float rstd = rsqrtf(group_sum(q, blockDim.x, red, slot) * inv + a.eps);
+        const float rstd = rsqrtf(block_sum(q, red, slot) * inv + a.eps);
         if (threadIdx.x == 0 && a.mean) {
             a.mean[r] = mu;
             a.rstd[r] = rstd;
@@ -261,8 +424,8 @@ __global__ void __launch_bounds__(1024) wide_backward_kernel(const Args a) {
             s1 += v;
             s2 += v * ((to_f32(x[c]) - mu) * rstd);
         }
-        s1 = group_sum(s1, blockDim.x, red, slot) * inv;
-        s2 = group_sum(s2, blockDim.x, red, slot) * inv;
+        s1 = block_sum(s1, red, slot) * inv;
+        s2 = block_sum(s2, red, slot) * inv;
         for (int c = threadIdx.x; c < a.width; c += blockDim.x) {
             const float v = to_f32(g[c]) * (a.w ? param_at<T>(a.w, a.param_f32, c) : 1.0f);
             gx[c] = from_f32<T>(rstd * (v - s1 - (to_f32(x[c]) - mu) * rstd * s2));
@@ -286,16 +449,58 @@ __global__ void __launch_bounds__(kBlock) wide_columns_kernel(const Args a) {
     out[a.width + c] = sb;
 }
 
-// Elements a thread: 8 while a row fits one warp that way (more rows in flight, fewer registers),
-// else 16.
-int elems_per_thread(int width) { return width <= 8 * 32 ? 8 : 16; }
+// How a row is spread: vectors of `vec` elements, `elems` elements a thread, `tpr` threads a row.
+// Vectors are 16 bytes where every row of every tensor starts equally far behind a 16-byte boundary
+// (then `shift` unless that is 0), else as wide as the addresses allow.  16 elements a thread, so that
+// the sums across threads are a small part of the work, but 8 in short rows, where 16 would leave
+// fewer than 4 threads side by side on a row.
+struct Spread {
+    int vec, elems, tpr, threads;
+    bool shift;
+};
 
-// Blocks of the backward: one wave at two blocks a SM, so that the partial sums stay few.
-int64_t backward_blocks(int64_t rows, int width) {
+struct RowsAt {
+    const void *p;
+    int64_t stride;
+};
+
+template <int N>
+Spread spread(const RowsAt (&t)[N], int width, size_t es) {
+    Spread s = {};
+    uint64_t bits = (uint64_t)width * es;
+    bool together = true;
+    for (int i = 0; i < N; i++) {
+        if (!t[i].p) continue;
+        bits |= (uint64_t)reinterpret_cast<uintptr_t>(t[i].p) | (uint64_t)t[i].stride * es;
+        together &= ((reinterpret_cast<uintptr_t>(t[i].p) ^ reinterpret_cast<uintptr_t>(t[0].p)) & 15) == 0 &&
+                    ((uint64_t)(t[i].stride - t[0].stride) * es & 15) == 0;
+    }
+    const int whole = (int)(16 / es);
+    s.vec = vector_elems(bits, es);
+    s.shift = s.vec < whole && together;
+    if (s.shift) s.vec = whole;
+    const int reach = width + (s.shift ? whole - 1 : 0);
+    s.elems = reach <= 64 ? 8 : 16;
+    s.tpr = pow2_ceil((reach + s.elems - 1) / s.elems);
+    s.threads = s.tpr > kBlock ? s.tpr : kBlock;
+    return s;
+}
+
+// The ring of one tensor: kStages parts of a row for each thread, where vectors are 16 bytes.
+size_t ring_bytes(const Spread &s, size_t es) {
+    return s.vec * es == 16 ? (size_t)kStages * (s.elems / s.vec) * s.threads * 16 : 0;
+}
+
+// Blocks that give every thread group rows a multiple of 8 apart (equal row shifts).
+int64_t blocks_of(int64_t rows, int groups, int64_t most) {
+    return (min64((rows + groups - 1) / groups, most) + 7) / 8 * 8;
+}
+
+// Blocks of the backward: about one wave, so that the partial sums stay few.
+constexpr int64_t kBackwardBlocks = 148 * 2;
+int64_t backward_blocks(int64_t rows, int width, int groups) {
     if (width > kMaxWidth) return min64(max64(rows / 8, 1), 64);
-    const int tpr = pow2_ceil((width + elems_per_thread(width) - 1) / elems_per_thread(width));
-    const int groups = tpr > kBlock ? 1 : kBlock / tpr;
-    return max64(1, min64((rows + groups - 1) / groups, 148 * 2));
+    return blocks_of(rows, groups, kBackwardBlocks);
 }
 
 }  // namespace lnorm
@@ -306,7 +511,7 @@ using namespace feq::token;
 
 extern "C" size_t feq_layer_norm_bwd_workspace_bytes(int64_t rows, int32_t width) {
     if (rows <= 0 || width <= 0) return 0;
-    return (size_t)lnorm::backward_blocks(rows, width) * 2 * (size_t)width * sizeof(float);
+    return (size_t)lnorm::backward_blocks(rows, width, 1) * 2 * (size_t)width * sizeof(float);
 }
 
 extern "C" int feq_layer_norm_fwd(const void *x, int64_t rows, int64_t x_stride, int32_t width, int32_t dtype,
@@ -337,16 +542,31 @@ extern "C" int feq_layer_norm_fwd(const void *x, int64_t rows, int64_t x_stride,
         FEQ_LAUNCH_CHECK();
         return FEQ_OK;
     }
-    const int vec = vector_elems((uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)y | (uint64_t)x_stride * es |
-                                     (uint64_t)width * es, es);
-    const int elems = lnorm::elems_per_thread(width);
-    a.tpr = pow2_ceil((width + elems - 1) / elems);
-    const int threads = a.tpr > lnorm::kBlock ? a.tpr : lnorm::kBlock, groups = threads / a.tpr;
-    const unsigned grid = (unsigned)min64((rows + groups - 1) / groups, (int64_t)sm_count() * (2048 / threads));
-    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, if (elems == 8) lnorm::forward_kernel<T, V, 8><<<grid, threads, 0, s>>>(a);
-                                        else lnorm::forward_kernel<T, V, 16><<<grid, threads, 0, s>>>(a);))
-    FEQ_LAUNCH_CHECK();
-    return FEQ_OK;
+    const lnorm::RowsAt at[2] = {{x, x_stride}, {y, width}};
+    const lnorm::Spread sp = lnorm::spread(at, width, es);
+    a.tpr = sp.tpr;
+    const int groups = sp.threads / sp.tpr;
+    const unsigned grid = (unsigned)lnorm::blocks_of(rows, groups, (int64_t)sm_count() * (1024 / sp.threads));
+    const size_t smem = lnorm::ring_bytes(sp, es);
+    auto go = [&](auto kern) -> int {
+        if (smem > 48 * 1024 - 1024)
+            FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kern<<<grid, sp.threads, smem, s>>>(a);
+        FEQ_LAUNCH_CHECK();
+        return FEQ_OK;
+    };
+    int rc = FEQ_OK;
+    FEQ_TOKEN_TYPE(dtype, {
+        constexpr int W = 16 / sizeof(T);
+        if (sp.shift) {
+            rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, W, 8, true> : lnorm::forward_kernel<T, W, 16, true>);
+        } else {
+            FEQ_TOKEN_VEC(T, sp.vec, {
+                rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, V, 8, false> : lnorm::forward_kernel<T, V, 16, false>);
+            })
+        }
+    })
+    return rc;
 }
 
 extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, const void *x, int64_t rows,
@@ -383,8 +603,9 @@ extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, con
     a.g_stride = grad_stride;
     a.width = width;
     a.param_f32 = param_f32;
-    const int blocks = (int)lnorm::backward_blocks(rows, width);
+    int blocks;
     if (width > lnorm::kMaxWidth) {
+        blocks = (int)lnorm::backward_blocks(rows, width, 1);
         if (grad_x) {
             const unsigned grid = (unsigned)min64(rows, sm_count() * 2);
             FEQ_TOKEN_TYPE(dtype, lnorm::wide_backward_kernel<T><<<grid, 1024, 0, s>>>(a);)
@@ -396,20 +617,30 @@ extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, con
             FEQ_LAUNCH_CHECK();
         }
     } else {
-        const int vec = vector_elems((uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)grad_out |
-                                         (uint64_t)(uintptr_t)grad_x | (uint64_t)x_stride * es |
-                                         (uint64_t)grad_stride * es | (uint64_t)width * es, es);
-        const int elems = lnorm::elems_per_thread(width);
-        a.tpr = pow2_ceil((width + elems - 1) / elems);
-        const int threads = a.tpr > lnorm::kBlock ? a.tpr : lnorm::kBlock;
-        const size_t smem = params ? (size_t)width * 2 * sizeof(float) : 0;
-        FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, {
-            auto kern = elems == 8 ? lnorm::backward_kernel<T, V, 8> : lnorm::backward_kernel<T, V, 16>;
-            if (smem > 40 * 1024)
+        const lnorm::RowsAt at[3] = {{x, x_stride}, {grad_out, grad_stride}, {grad_x, width}};
+        const lnorm::Spread sp = lnorm::spread(at, width, es);
+        a.tpr = sp.tpr;
+        blocks = (int)lnorm::backward_blocks(rows, width, sp.threads / sp.tpr);
+        const size_t smem = std::max(2 * lnorm::ring_bytes(sp, es), params ? (size_t)width * 2 * sizeof(float) : 0);
+        auto go = [&](auto kern) -> int {
+            if (smem > 48 * 1024 - 1024)
                 FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            kern<<<(unsigned)blocks, threads, smem, s>>>(a);
-        }))
-        FEQ_LAUNCH_CHECK();
+            kern<<<(unsigned)blocks, sp.threads, smem, s>>>(a);
+            FEQ_LAUNCH_CHECK();
+            return FEQ_OK;
+        };
+        int rc = FEQ_OK;
+        FEQ_TOKEN_TYPE(dtype, {
+            constexpr int W = 16 / sizeof(T);
+            if (sp.shift) {
+                rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, W, 8, true> : lnorm::backward_kernel<T, W, 16, true>);
+            } else {
+                FEQ_TOKEN_VEC(T, sp.vec, {
+                    rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, V, 8, false> : lnorm::backward_kernel<T, V, 16, false>);
+                })
+            }
+        })
+        if (rc != FEQ_OK) return rc;
     }
     if (params) {
         const unsigned grid = (unsigned)((2 * (int64_t)width + lnorm::kReduceCols - 1) / lnorm::kReduceCols);

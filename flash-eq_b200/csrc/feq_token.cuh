@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "feq_internal.cuh"
 
 namespace feq {
@@ -69,8 +71,12 @@ inline int pow2_ceil(int64_t n) {
 }
 
 inline int sm_count() {
+    static std::atomic<int> known[64];       // by device; 0: not asked yet
     int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (cudaGetDevice(&dev) != cudaSuccess) return sms;
+    if (dev >= 0 && dev < 64 && known[dev].load(std::memory_order_relaxed)) return known[dev].load(std::memory_order_relaxed);
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && dev >= 0 && dev < 64)
+        known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 

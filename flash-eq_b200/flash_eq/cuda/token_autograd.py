@@ -19,7 +19,9 @@ from . import token_ops
 
 
 def _tracks(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    return any(t is not None and t.requires_grad for t in tensors)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -129,7 +131,7 @@ def expert_dispatch(x: torch.Tensor, route: ExpertRoute) -> torch.Tensor:
         out = _Dispatch.apply(rows, route.slots, route.offsets)
     else:
         out = token_ops.expert_dispatch(rows, route.slots, route.offsets)
-    return out.view(out.shape[0], *x.shape[1:])
+    return out if x.dim() == 2 else out.view(out.shape[0], *x.shape[1:])
 
 
 class _Combine(torch.autograd.Function):
@@ -154,7 +156,7 @@ def expert_combine(y: torch.Tensor, route: ExpertRoute) -> torch.Tensor:
         out = _Combine.apply(rows, route.weights, route.slots, route.offsets)
     else:
         out = token_ops.expert_combine(rows, route.slots, route.offsets, route.weights)
-    return out.view(out.shape[0], *y.shape[1:])
+    return out if y.dim() == 2 else out.view(out.shape[0], *y.shape[1:])
 
 
 class _ExpertLinear(torch.autograd.Function):
@@ -181,16 +183,8 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     Equivariant rows: x (rows, dim, c_in) with dim = sum(2 l + 1) over ``lvals``, weight (num_experts,
     len(lvals), c_out, c_in), bias (num_experts, number of l = 0 irreps, c_out) on the l = 0
     components.  float32, bfloat16 or float16, one type for all; sums in float32."""
-    lvals = tuple(int(v) for v in lvals)
-    plain = x.dim() == 2
-    if plain:
-        if lvals != (0,) or weight.dim() != 3 or (bias is not None and bias.dim() != 2):
-            raise ValueError("plain rows (rows, c_in) need weight (num_experts, c_out, c_in), bias (num_experts, "
-                             f"c_out) and lvals (0,); got {tuple(weight.shape)}, lvals {list(lvals)}")
-        x, weight = x.unsqueeze(1), weight.unsqueeze(1)
-        bias = None if bias is None else bias.unsqueeze(1)
+    if type(lvals) is not tuple:
+        lvals = tuple(int(v) for v in lvals)
     if _tracks(x, weight, bias):
-        y = _ExpertLinear.apply(x, weight, bias, offsets, lvals)
-    else:
-        y = token_ops.expert_linear_fwd(x, weight, bias, offsets, lvals)
-    return y.squeeze(1) if plain else y
+        return _ExpertLinear.apply(x, weight, bias, offsets, lvals)
+    return token_ops.expert_linear_fwd(x, weight, bias, offsets, lvals)

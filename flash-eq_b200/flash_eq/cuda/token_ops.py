@@ -1,23 +1,55 @@
 """Torch-facing wrappers of the layer norm and mixture-of-experts kernels (csrc/feq_layernorm.cu,
 csrc/feq_experts.cu, csrc/feq_expertlin.cu).
 
-Like ``ops``: inputs are checked, outputs and workspace come from torch's caching allocator and the
+As in ``ops``: inputs are checked, outputs and workspace come from torch's caching allocator and the
 kernels are enqueued on the current stream of the inputs' device; no host synchronisation.
 Element types: float32, bfloat16, float16.  The last dimension is read contiguous, rows may
 be strided; anything else is copied first.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .ops import _p, _require_cuda, _stream, _workspace
+from .ops import _require_cuda
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_EXPERTS, MAX_TOP_K = 512, 32
+
+# These wrappers run in front of kernels of a few microseconds, so they pass plain integers to ctypes and
+# ask torch for a stream handle without building a Stream object.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _ready(first: torch.Tensor, *others):
+    """The library, after checking that every tensor lies on one CUDA device."""
+    dev = first.get_device()
+    if dev < 0 or any(t is not None and t.get_device() != dev for t in others):
+        _require_cuda(first, *others)
+        raise RuntimeError("flash-eq ops need all tensors on one device; got "
+                           + ", ".join(str(t.device) for t in (first, *others) if t is not None))
+    return _lib.load()
+
+
+def _call(fn, what: str, dev: int, *args) -> None:
+    """fn(*args, stream) with ``dev`` current, on its current stream."""
+    rc = _call_rc(fn, dev, *args)
+    if rc:
+        _lib.check(rc, what)
+
+
+def _call_rc(fn, dev: int, *args) -> int:
+    if dev == torch.cuda.current_device():
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
+
+
+def _ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
@@ -27,33 +59,23 @@ def _dtype(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _same_device(first: torch.Tensor, *others) -> None:
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise RuntimeError(f"flash-eq ops need all tensors on one device; got {first.device} and {t.device}")
-
-
-def _on(device):
-    """Context that makes ``device`` current for the launches (a no-op when it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """(rows, width) with a contiguous last dimension."""
-    t = t.detach()
     return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _param(p, like: torch.Tensor, width: int, name: str):
     if p is None:
         return None
-    if p.shape != (width,):
+    if p.dim() != 1 or p.shape[0] != width:
         raise ValueError(f"{name} must have shape ({width},); got {tuple(p.shape)}")
-    if p.dtype not in (like.dtype, torch.float32):
+    if p.dtype is not like.dtype and p.dtype is not torch.float32:
         raise TypeError(f"{name} must be {like.dtype} or float32; got {p.dtype}")
-    return p.detach().contiguous()
+    return p.contiguous()
+
+
+def _workspace(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 # ---------------------------------------------------------------------------
@@ -61,38 +83,35 @@ def _param(p, like: torch.Tensor, width: int, name: str):
 # ---------------------------------------------------------------------------
 def layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, keep_stats: bool):
     """(y, mean, rstd) of x (..., D); mean / rstd None unless ``keep_stats``."""
-    lib = _require_cuda(x, weight, bias)
-    _same_device(x, weight, bias)
+    lib = _ready(x, weight, bias)
     code = _dtype(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
+    width = x.shape[-1] if x.dim() else 0
+    if width < 1:
         raise ValueError(f"x must have a last dimension of at least 1; got {tuple(x.shape)}")
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError(f"eps must be >= 0; got {eps}")
-    width = x.shape[-1]
     weight, bias = _param(weight, x, width, "weight"), _param(bias, x, width, "bias")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise TypeError(f"weight and bias must have one type; got {weight.dtype} and {bias.dtype}")
-    rows = _rows(x.reshape(-1, width))
-    n = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rows = _rows(x if x.dim() == 2 else x.reshape(-1, width))
+    n, dev = rows.shape[0], x.device
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     mean = rstd = None
     if keep_stats:
-        mean, rstd = torch.empty(2, n, dtype=torch.float32, device=x.device)
-    p = weight if weight is not None else bias
-    with _on(x.device):
-        rc = lib.feq_layer_norm_fwd(_p(rows), n, rows.stride(0), width, code, _p(weight), _p(bias),
-                                    int(p is not None and p.dtype == torch.float32), eps, _p(y), _p(mean), _p(rstd),
-                                    _stream(x.device))
-    _lib.check(rc, "feq_layer_norm_fwd")
+        mean = torch.empty(n, dtype=torch.float32, device=dev)
+        rstd = torch.empty(n, dtype=torch.float32, device=dev)
+    p = bias if weight is None else weight
+    _call(lib.feq_layer_norm_fwd, "feq_layer_norm_fwd", dev.index, rows.data_ptr(), n, rows.stride(0), width, code,
+          _ptr(weight), _ptr(bias), int(p is not None and p.dtype is torch.float32), eps, y.data_ptr(), _ptr(mean),
+          _ptr(rstd))
     return y, mean, rstd
 
 
 def layer_norm_bwd(grad_out, x, weight, mean, rstd, need_x=True, need_weight=True, need_bias=True, param_dtype=None):
     """(grad_x, grad_weight, grad_bias) of ``layer_norm_fwd``; None where not needed."""
-    lib = _require_cuda(grad_out, x, weight)
-    code = _dtype(x, "x")
-    width = x.shape[-1]
+    lib = _ready(grad_out, x, weight)
+    code, width = _dtype(x, "x"), x.shape[-1]
     weight = _param(weight, x, width, "weight")
     rows, g = _rows(x.reshape(-1, width)), _rows(grad_out.reshape(-1, width))
     n, dev = rows.shape[0], x.device
@@ -100,12 +119,11 @@ def layer_norm_bwd(grad_out, x, weight, mean, rstd, need_x=True, need_weight=Tru
     gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
     gw = torch.empty(width, dtype=pd, device=dev) if need_weight else None
     gb = torch.empty(width, dtype=pd, device=dev) if need_bias else None
-    ws = _workspace(lib.feq_layer_norm_bwd_workspace_bytes(n, width), dev) if need_weight or need_bias else None
-    with _on(dev):
-        rc = lib.feq_layer_norm_bwd(_p(g), g.stride(0), _p(rows), n, rows.stride(0), width, code, _p(weight),
-                                    int(pd == torch.float32), _p(mean), _p(rstd), _p(gx), _p(gw), _p(gb), _p(ws),
-                                    0 if ws is None else ws.numel(), _stream(dev))
-    _lib.check(rc, "feq_layer_norm_bwd")
+    nbytes = lib.feq_layer_norm_bwd_workspace_bytes(n, width) if need_weight or need_bias else 0
+    ws = _workspace(nbytes, dev)
+    _call(lib.feq_layer_norm_bwd, "feq_layer_norm_bwd", dev.index, g.data_ptr(), g.stride(0), rows.data_ptr(), n,
+          rows.stride(0), width, code, _ptr(weight), int(pd is torch.float32), mean.data_ptr(), rstd.data_ptr(),
+          _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes)
     return gx, gw, gb
 
 
@@ -114,7 +132,7 @@ def layer_norm_bwd(grad_out, x, weight, mean, rstd, need_x=True, need_weight=Tru
 # ---------------------------------------------------------------------------
 def expert_route(logits: torch.Tensor, top_k: int, normalize: bool = True):
     """(experts, weights, slots, offsets) of logits (tokens, num_experts)."""
-    lib = _require_cuda(logits)
+    lib = _ready(logits)
     code = _dtype(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"logits must be (tokens, num_experts); got {tuple(logits.shape)}")
@@ -125,186 +143,180 @@ def expert_route(logits: torch.Tensor, top_k: int, normalize: bool = True):
     if e > MAX_EXPERTS or k > MAX_TOP_K:
         raise ValueError(f"at most {MAX_EXPERTS} experts and top_k {MAX_TOP_K}; got {e} and {k}")
     rows, dev = _rows(logits), logits.device
-    ids, slots = torch.empty(2, n, k, dtype=torch.int32, device=dev)
+    ids = torch.empty(n, k, dtype=torch.int32, device=dev)
+    slots = torch.empty(n, k, dtype=torch.int32, device=dev)
     weights = torch.empty(n, k, dtype=torch.float32, device=dev)
     offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
-    ws = _workspace(lib.feq_expert_route_workspace_bytes(n, k, e), dev)
-    with _on(dev):
-        rc = lib.feq_expert_route(_p(rows), n, rows.stride(0), e, k, code, int(bool(normalize)), _p(ids), _p(weights),
-                                  _p(slots), _p(offsets), _p(ws), ws.numel(), _stream(dev))
-    _lib.check(rc, "feq_expert_route")
+    nbytes = lib.feq_expert_route_workspace_bytes(n, k, e)
+    ws = _workspace(nbytes, dev)
+    _call(lib.feq_expert_route, "feq_expert_route", dev.index, rows.data_ptr(), n, rows.stride(0), e, k, code,
+          int(bool(normalize)), ids.data_ptr(), weights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), _ptr(ws),
+          nbytes)
     return ids, weights, slots, offsets
 
 
 def expert_route_bwd(logits, ids, weights, grad_weights, normalize):
-    lib = _require_cuda(logits, grad_weights)
+    lib = _ready(logits, grad_weights)
     n, e = logits.shape
     rows, dev = _rows(logits), logits.device
-    grad_weights = grad_weights.detach().to(torch.float32).contiguous()
+    grad_weights = grad_weights.to(torch.float32).contiguous()
     out = torch.empty(n, e, dtype=logits.dtype, device=dev)
-    with _on(dev):
-        rc = lib.feq_expert_route_bwd(_p(rows), n, rows.stride(0), e, ids.shape[1], _dtype(logits, "logits"),
-                                      int(bool(normalize)), _p(ids), _p(weights), _p(grad_weights), _p(out),
-                                      _stream(dev))
-    _lib.check(rc, "feq_expert_route_bwd")
+    _call(lib.feq_expert_route_bwd, "feq_expert_route_bwd", dev.index, rows.data_ptr(), n, rows.stride(0), e,
+          ids.shape[1], _dtype(logits, "logits"), int(bool(normalize)), ids.data_ptr(), weights.data_ptr(),
+          grad_weights.data_ptr(), out.data_ptr())
     return out
 
 
 def _plan(slots: torch.Tensor, offsets: torch.Tensor):
-    if slots.dtype != torch.int32 or slots.dim() != 2 or not slots.is_contiguous():
+    if slots.dtype is not torch.int32 or slots.dim() != 2 or not slots.is_contiguous():
         raise TypeError("slots must be a contiguous int32 (tokens, top_k) tensor")
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2 or not offsets.is_contiguous():
+    if offsets.dtype is not torch.int32 or offsets.dim() != 1 or offsets.shape[0] < 2 or not offsets.is_contiguous():
         raise TypeError("offsets must be a contiguous int32 (num_experts + 1,) tensor")
-    return slots.shape[0], slots.shape[1], offsets.shape[0] - 1
+    return (*slots.shape, offsets.shape[0] - 1)
 
 
 def expert_dispatch(x: torch.Tensor, slots, offsets) -> torch.Tensor:
     """x (tokens, width) -> (tokens * top_k, width) sorted by expert."""
-    lib = _require_cuda(x, slots, offsets)
-    _same_device(x, slots, offsets)
+    lib = _ready(x, slots, offsets)
     n, k, e = _plan(slots, offsets)
     if x.dim() != 2 or x.shape[0] != n or x.shape[1] < 1:
         raise ValueError(f"x must be ({n}, width); got {tuple(x.shape)}")
-    code, rows = _dtype(x, "x"), _rows(x)
-    out = torch.empty(n * k, x.shape[1], dtype=x.dtype, device=x.device)
-    with _on(x.device):
-        rc = lib.feq_expert_dispatch(_p(rows), n, rows.stride(0), x.shape[1], code, k, e, _p(slots), _p(offsets),
-                                     _p(out), _stream(x.device))
-    _lib.check(rc, "feq_expert_dispatch")
+    code, rows, width = _dtype(x, "x"), _rows(x), x.shape[1]
+    out = torch.empty(n * k, width, dtype=x.dtype, device=x.device)
+    _call(lib.feq_expert_dispatch, "feq_expert_dispatch", x.device.index, rows.data_ptr(), n, rows.stride(0), width,
+          code, k, e, slots.data_ptr(), offsets.data_ptr(), out.data_ptr())
     return out
 
 
-def _sorted_rows(y, n, k, name):
+def _sorted_rows(y, n, k):
     if y.dim() != 2 or y.shape[0] != n * k or y.shape[1] < 1:
-        raise ValueError(f"{name} must be ({n * k}, width); got {tuple(y.shape)}")
+        raise ValueError(f"y must be ({n * k}, width); got {tuple(y.shape)}")
     return _rows(y)
 
 
 def expert_combine(y: torch.Tensor, slots, offsets, weights=None) -> torch.Tensor:
     """Sorted rows (tokens * top_k, width) -> (tokens, width), weighted by ``weights`` (tokens, top_k)."""
-    lib = _require_cuda(y, slots, offsets, weights)
-    _same_device(y, slots, offsets, weights)
+    lib = _ready(y, slots, offsets, weights)
     n, k, e = _plan(slots, offsets)
-    code, rows = _dtype(y, "y"), _sorted_rows(y, n, k, "y")
+    code, rows, width = _dtype(y, "y"), _sorted_rows(y, n, k), y.shape[1]
     if weights is not None:
-        if weights.shape != (n, k) or weights.dtype != torch.float32:
+        if weights.shape != slots.shape or weights.dtype is not torch.float32:
             raise ValueError(f"weights must be a float32 ({n}, {k}) tensor; got {weights.dtype} {tuple(weights.shape)}")
-        weights = weights.detach().contiguous()
-    out = torch.empty(n, y.shape[1], dtype=y.dtype, device=y.device)
-    with _on(y.device):
-        rc = lib.feq_expert_combine(_p(rows), rows.stride(0), n, y.shape[1], code, k, e, _p(slots), _p(offsets),
-                                    _p(weights), _p(out), _stream(y.device))
-    _lib.check(rc, "feq_expert_combine")
+        weights = weights.contiguous()
+    out = torch.empty(n, width, dtype=y.dtype, device=y.device)
+    _call(lib.feq_expert_combine, "feq_expert_combine", y.device.index, rows.data_ptr(), rows.stride(0), n, width,
+          code, k, e, slots.data_ptr(), offsets.data_ptr(), _ptr(weights), out.data_ptr())
     return out
 
 
 def expert_combine_bwd(grad_out, y, slots, offsets, weights):
     """(grad_y, grad_weights) of ``expert_combine`` with weights."""
-    lib = _require_cuda(grad_out, y, slots, offsets, weights)
+    lib = _ready(grad_out, y, slots, offsets, weights)
     n, k, e = _plan(slots, offsets)
-    code, rows, g = _dtype(y, "y"), _sorted_rows(y, n, k, "y"), _rows(grad_out)
-    gy = torch.empty(n * k, y.shape[1], dtype=y.dtype, device=y.device)
+    code, rows, g, width = _dtype(y, "y"), _sorted_rows(y, n, k), _rows(grad_out), y.shape[1]
+    gy = torch.empty(n * k, width, dtype=y.dtype, device=y.device)
     gw = torch.empty(n, k, dtype=torch.float32, device=y.device)
-    weights = weights.detach().contiguous()
-    with _on(y.device):
-        rc = lib.feq_expert_combine_bwd(_p(g), g.stride(0), _p(rows), rows.stride(0), n, y.shape[1], code, k, e,
-                                        _p(slots), _p(offsets), _p(weights), _p(gy), _p(gw), _stream(y.device))
-    _lib.check(rc, "feq_expert_combine_bwd")
+    weights = weights.contiguous()
+    _call(lib.feq_expert_combine_bwd, "feq_expert_combine_bwd", y.device.index, g.data_ptr(), g.stride(0),
+          rows.data_ptr(), rows.stride(0), n, width, code, k, e, slots.data_ptr(), offsets.data_ptr(),
+          weights.data_ptr(), gy.data_ptr(), gw.data_ptr())
     return gy, gw
 
 
 # ---------------------------------------------------------------------------
 # expert linear
 # ---------------------------------------------------------------------------
-def _dim(lvals) -> int:
-    return sum(2 * v + 1 for v in lvals)
+@functools.lru_cache(maxsize=64)
+def _degrees(lvals):
+    """(dim, number of l = 0 irreps, ctypes array) of a tuple of degrees."""
+    if not lvals or any(v < 0 for v in lvals):
+        raise ValueError(f"lvals must be a non-empty list of degrees >= 0; got {list(lvals)}")
+    return sum(2 * v + 1 for v in lvals), sum(v == 0 for v in lvals), _lib.i32_array(lvals)[0]
 
 
 def _strided(t: torch.Tensor) -> torch.Tensor:
-    t = t.detach()
-    return t if t.stride(2) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
-def check_expert_linear(x, weight, bias, offsets, lvals):
-    """Shapes of ``expert_linear``: x (rows, dim, c_in), weight (E, reps, c_out, c_in), bias (E, scalars, c_out)."""
-    _dtype(x, "x")
-    if not lvals or any(v < 0 for v in lvals):
-        raise ValueError(f"lvals must be a non-empty list of degrees >= 0; got {list(lvals)}")
-    dim, scalars = _dim(lvals), sum(v == 0 for v in lvals)
-    if x.dim() != 3 or x.shape[1] != dim or x.shape[2] < 1:
+def _linear_args(x, weight, offsets, lvals):
+    """Shapes of ``expert_linear``, and the arguments that both directions share.
+
+    x (rows, dim, c_in) with weight (E, reps, c_out, c_in), or plain x (rows, c_in) with (E, c_out, c_in)."""
+    code = _dtype(x, "x")
+    dim, scalars, arr = _degrees(lvals)
+    plain = x.dim() == 2
+    if plain:
+        if lvals != (0,):
+            raise ValueError(f"plain rows (rows, c_in) need lvals (0,); got {list(lvals)}")
+    elif x.dim() != 3 or x.shape[1] != dim:
         raise ValueError(f"x must be (rows, {dim}, c_in) for lvals {list(lvals)}; got {tuple(x.shape)}")
-    if weight.dim() != 4 or weight.shape[1] != len(lvals) or weight.shape[3] != x.shape[2] or weight.shape[2] < 1 \
-            or weight.shape[0] < 1:
-        raise ValueError(f"weight must be (num_experts, {len(lvals)}, c_out, {x.shape[2]}); got {tuple(weight.shape)}")
-    e, co = weight.shape[0], weight.shape[2]
+    ci = x.shape[-1]
+    shape = weight.shape
+    if len(shape) != (3 if plain else 4) or shape[-1] != ci or ci < 1 or shape[-2] < 1 or shape[0] < 1 or not (
+            plain or shape[1] == len(lvals)):
+        want = "(num_experts, c_out, " if plain else f"(num_experts, {len(lvals)}, c_out, "
+        raise ValueError(f"weight must be {want}{ci}); got {tuple(shape)}")
+    e, co = shape[0], shape[-2]
     if e > MAX_EXPERTS:
         raise ValueError(f"at most {MAX_EXPERTS} experts; got {e}")
-    if weight.dtype != x.dtype:
+    if weight.dtype is not x.dtype:
         raise TypeError(f"weight must have x's type {x.dtype}; got {weight.dtype}")
-    if bias is not None:
-        if scalars == 0:
-            raise ValueError(f"a bias needs an l = 0 component; lvals are {list(lvals)}")
-        if bias.shape != (e, scalars, co):
-            raise ValueError(f"bias must be ({e}, {scalars}, {co}); got {tuple(bias.shape)}")
-        if bias.dtype != x.dtype:
-            raise TypeError(f"bias must have x's type {x.dtype}; got {bias.dtype}")
     if offsets.dim() != 1 or offsets.shape[0] != e + 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"offsets must be an int32 or int64 ({e + 1},) tensor; got {offsets.dtype} {tuple(offsets.shape)}")
-    _same_device(x, weight, bias, offsets)
+    # kept alive by the caller until the call has returned
+    x, weight = _strided(x), weight.contiguous()
+    offsets = (offsets if offsets.dtype is torch.int32 else offsets.to(torch.int32)).contiguous()
+    a = _lib.FeqExpertLinearArgs(x.data_ptr(), x.stride(0), 0 if plain else x.stride(1), weight.data_ptr(), None,
+                                 offsets.data_ptr(), x.shape[0], arr, len(lvals), e, ci, co, code)
+    return a, (x, weight, offsets), scalars
 
 
-def _linear_args(x, weight, offsets, lvals, status):
-    a = _lib.FeqExpertLinearArgs()
-    arr, a.n_lvals = _lib.i32_array(lvals)
-    a.lvals = ctypes.cast(arr, _lib.c_i32p)
-    a.weight, a.offsets = weight.data_ptr(), offsets.data_ptr()
-    a.num_experts, _, a.c_out, a.c_in = weight.shape
-    a.dtype = DTYPES[weight.dtype]
-    if x is not None:
-        a.x, a.rows, a.x_row_stride, a.x_comp_stride = x.data_ptr(), x.shape[0], x.stride(0), x.stride(1)
+def _run_linear(lib, fn, what, a, backward, device, status):
     if status is not None:
         a.status = status.data_ptr()
-    return a, arr
-
-
-def _linear_workspace(lib, a, backward, device):
-    nbytes = lib.feq_expert_linear_workspace_bytes(ctypes.byref(a), backward)
-    if nbytes == 0:
-        raise RuntimeError("expert_linear: unsupported shape (l <= 16, <= 64 irreps, dim <= 512, < 2^31 rows)")
-    return _workspace(nbytes, device)
+    ref = ctypes.byref(a)
+    rc = _call_rc(fn, device.index, ref, None, 0)
+    if rc == _lib.FEQ_ERR_WORKSPACE:          # an operand has to be packed, or sums joined
+        nbytes = lib.feq_expert_linear_workspace_bytes(ref, backward)
+        ws = _workspace(nbytes, device)
+        rc = _call_rc(fn, device.index, ref, _ptr(ws), nbytes)
+    if rc:
+        _lib.check(rc, what)
 
 
 def expert_linear_fwd(x, weight, bias, offsets, lvals, status=None) -> torch.Tensor:
-    lib = _require_cuda(x, weight, bias, offsets)
-    check_expert_linear(x, weight, bias, offsets, lvals)
-    x, weight = _strided(x), weight.detach().contiguous()
-    bias = None if bias is None else bias.detach().contiguous()
-    offsets = offsets.to(torch.int32).contiguous()
-    out = torch.empty(x.shape[0], x.shape[1], weight.shape[2], dtype=x.dtype, device=x.device)
-    a, keep = _linear_args(x, weight, offsets, lvals, status)
+    lib = _ready(x, weight, bias, offsets)
+    a, kept, scalars = _linear_args(x, weight, offsets, lvals)
+    plain = x.dim() == 2
+    if bias is not None:
+        if scalars == 0:
+            raise ValueError(f"a bias needs an l = 0 component; lvals are {list(lvals)}")
+        want = (a.num_experts, a.c_out) if plain else (a.num_experts, scalars, a.c_out)
+        if bias.shape != want:
+            raise ValueError(f"bias must be {want}; got {tuple(bias.shape)}")
+        if bias.dtype is not x.dtype:
+            raise TypeError(f"bias must have x's type {x.dtype}; got {bias.dtype}")
+        bias = bias.contiguous()
+        a.bias = bias.data_ptr()
+    out = torch.empty((x.shape[0], a.c_out) if plain else (x.shape[0], x.shape[1], a.c_out), dtype=x.dtype,
+                      device=x.device)
     a.out = out.data_ptr()
-    a.bias = None if bias is None else bias.data_ptr()
-    with _on(x.device):
-        ws = _linear_workspace(lib, a, 0, x.device)
-        rc = lib.feq_expert_linear_fwd(ctypes.byref(a), _p(ws), ws.numel(), _stream(x.device))
-    _lib.check(rc, "feq_expert_linear_fwd")
+    _run_linear(lib, lib.feq_expert_linear_fwd, "feq_expert_linear_fwd", a, 0, x.device, status)
     return out
 
 
 def expert_linear_bwd(grad_out, x, weight, offsets, lvals, need_x=True, need_weight=True, need_bias=True, status=None):
     """(grad_x, grad_weight, grad_bias) of ``expert_linear_fwd``; None where not needed."""
-    lib = _require_cuda(grad_out, x, weight, offsets)
-    x, weight, g = _strided(x), weight.detach().contiguous(), _strided(grad_out)
-    offsets = offsets.to(torch.int32).contiguous()
-    dev, (e, reps, co, ci) = x.device, weight.shape
+    lib = _ready(grad_out, x, weight, offsets)
+    a, kept, scalars = _linear_args(x, weight, offsets, lvals)
+    g, dev, plain = _strided(grad_out), x.device, x.dim() == 2
     gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
     gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_weight else None
-    gb = torch.empty(e, sum(v == 0 for v in lvals), co, dtype=x.dtype, device=dev) if need_bias else None
-    a, keep = _linear_args(x, weight, offsets, lvals, status)
-    a.grad_out, a.grad_row_stride, a.grad_comp_stride = g.data_ptr(), g.stride(0), g.stride(1)
-    a.grad_x, a.grad_weight, a.grad_bias = (None if t is None else t.data_ptr() for t in (gx, gw, gb))
-    with _on(dev):
-        ws = _linear_workspace(lib, a, 1, dev)
-        rc = lib.feq_expert_linear_bwd(ctypes.byref(a), _p(ws), ws.numel(), _stream(dev))
-    _lib.check(rc, "feq_expert_linear_bwd")
+    gb = None
+    if need_bias:
+        gb = torch.empty((a.num_experts, a.c_out) if plain else (a.num_experts, scalars, a.c_out), dtype=x.dtype,
+                         device=dev)
+    a.grad_out, a.grad_row_stride, a.grad_comp_stride = g.data_ptr(), g.stride(0), 0 if plain else g.stride(1)
+    a.grad_x, a.grad_weight, a.grad_bias = _ptr(gx), _ptr(gw), _ptr(gb)
+    _run_linear(lib, lib.feq_expert_linear_bwd, "feq_expert_linear_bwd", a, 1, dev, status)
     return gx, gw, gb

@@ -570,7 +570,7 @@ int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, const void *x,
  * where a choice is missing; slots (tokens, top_k) = the place of every (token, choice) pair in the
  * stable order by expert, pairs without an expert last; offsets (num_experts + 1) = the first place
  * of each expert, offsets[num_experts] = the number of pairs that have one.  NaN counts as the
- * largest logit.  num_experts <= 512, top_k <= 32, tokens * top_k < 2^31. */
+ * largest logit.  No workspace is needed where _workspace_bytes says 0.  num_experts <= 512, top_k <= 32, tokens * top_k < 2^31. */
 size_t feq_expert_route_workspace_bytes(int64_t tokens, int32_t top_k, int32_t num_experts);
 int feq_expert_route(const void *logits, int64_t tokens, int64_t stride, int32_t num_experts, int32_t top_k,
                      int32_t dtype, int32_t normalize, int32_t *ids, float *weights, int32_t *slots, int32_t *offsets,
@@ -617,7 +617,8 @@ typedef struct {
     void *grad_x, *grad_weight, *grad_bias;
     int32_t *status;
 } FeqExpertLinearArgs;
-/* 0: the shape is not served. */
+/* Enough for the call with these arguments, addresses and strides included (0: not served).  A call
+ * that needs no workspace takes NULL; one that does returns FEQ_ERR_WORKSPACE before any work. */
 size_t feq_expert_linear_workspace_bytes(const FeqExpertLinearArgs *args, int32_t backward);
 int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *workspace, size_t workspace_bytes,
                           feq_stream_t stream);
