@@ -26,7 +26,7 @@ namespace lnorm {
 
 using namespace token;
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256;                  // threads of a block, unless a row takes kMaxTpr
 constexpr int kMaxTpr = 512;
 constexpr int kMaxWidth = 16 * kMaxTpr - 8;  // 16 elements a thread, the first up to 7 before the row
 constexpr int kLimitWidth = 1 << 29;         // column arithmetic stays in 32 bits
@@ -88,119 +88,144 @@ __device__ __forceinline__ void group_sum(float (&v)[K], int tpr, float (*red)[K
 // A thread's part of a row: N = E / V vectors, vector i covers the columns from (i * tpr + t) * V - shift on.
 // shift (kShift) is how far the row starts behind a 16-byte boundary, in elements: the vectors lie on
 // the boundary whatever the row's address, and the first and the last are moved by elements.
-template <int V>
-__device__ __forceinline__ int column(int e, int tpr, int t, int shift) { return (e / V * tpr + t) * V - shift + e % V; }
-
-// Bit e: element e of the thread is a column of the row.
-template <int V, int E>
-__device__ __forceinline__ uint32_t columns_of(int width, int tpr, int t, int shift) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        const int c = column<V>(e, tpr, t, shift);
-        if (c >= 0 && c < width) m |= 1u << e;
-    }
-    return m;
-}
-
 // Rows in flight.  16-byte vectors go through a ring in shared memory that each thread fills (cp.async)
 // and reads for itself, kAhead rows ahead, so that what is in flight takes no registers and needs no
-// barrier; narrower ones are loaded when they are used.
+// barrier; narrower ones are loaded when they are used.  Elements that are no column of a row (past
+// its end, or of a row past the last) read as 0.
 constexpr int kStages = 3, kAhead = kStages - 1;
 
 template <typename T, int V, int E, bool kShift>
 struct Stream {
     static constexpr bool kRing = V * sizeof(T) == 16;
     static constexpr int N = E / V;
-    uint8_t *ring;                            // kStages slots, `slot_bytes` apart
+    uint8_t *ring;                            // kStages slots, slot_bytes apart
     uint32_t slot_bytes;
-    const T *base;
-    int64_t stride, rows;
-    int width, tpr, t, shift;
+    const T *next;                            // the row to fetch, at the thread's first vector
+    int64_t step;                             // elements from a row of the group to its next
+    int64_t left;                             // rows of the group still to fetch
+    int width, c0, pitch;                     // c0: the first column of the thread; vectors `pitch` apart
 
-    __device__ __forceinline__ const T *row(int64_t r) const { return base + r * stride; }
-    __device__ __forceinline__ Pack<T, V> *slot(int s, int i) const {
-        return reinterpret_cast<Pack<T, V> *>(ring + s * slot_bytes + (i * blockDim.x + threadIdx.x) * 16);
-    }
-    __device__ __forceinline__ Pack<T, V> edge(const T *p, int c) const {      // some elements lie outside the row
-        Pack<T, V> d;
+    __device__ __forceinline__ Stream(uint8_t *ring_, uint32_t slot_bytes_, const void *base, int64_t first, int64_t every,
+                                      int64_t stride, const Args &a, int t, int shift)
+        : ring(ring_ + threadIdx.x * 16), slot_bytes(slot_bytes_), step(every * stride), width(a.width) {
+        c0 = t * V - (kShift ? shift : 0);
+        pitch = a.tpr * V;
+        next = static_cast<const T *>(base) + first * stride + c0;
+        left = first < a.rows ? (a.rows - first + every - 1) / every : 0;
+        if (kRing) {
 #pragma unroll
-        for (int q = 0; q < V; q++) d.v[q] = c + q >= 0 && c + q < width ? p[c + q] : from_f32<T>(0.0f);
-        return d;
-    }
-    __device__ __forceinline__ void fetch(int64_t r, int s) const {
-        if (!kRing || r >= rows) return;
-        const T *p = row(r);
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int c = (i * tpr + t) * V - (kShift ? shift : 0);
-            if (kShift ? c >= 0 && c + V <= width : c < width)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                 static_cast<uint32_t>(__cvta_generic_to_shared(slot(s, i)))), "l"(p + c) : "memory");
-            else if (kShift && c + V > 0 && c < width)
-                *slot(s, i) = edge(p, c);
+            for (int k = 0; k < kStages; k++) clear(k);
         }
     }
-    // zeros where the thread has no column
-    __device__ __forceinline__ void read(int64_t r, int s, float (&v)[E]) const {
+    __device__ __forceinline__ Pack<T, V> *slot(int s, int i) const {
+        return reinterpret_cast<Pack<T, V> *>(ring + s * slot_bytes + i * blockDim.x * 16);
+    }
+    __device__ __forceinline__ void clear(int s) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) *reinterpret_cast<uint4 *>(slot(s, i)) = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ bool whole(int i) const {
+        const int c = c0 + i * pitch;
+        return kShift ? c >= 0 && c + V <= width : c < width;
+    }
+    __device__ __forceinline__ Pack<T, V> edge(int i) const {      // some elements lie outside the row
+        const int c = c0 + i * pitch;
+        Pack<T, V> d;
+#pragma unroll
+        for (int q = 0; q < V; q++) d.v[q] = c + q >= 0 && c + q < width ? next[i * pitch + q] : from_f32<T>(0.0f);
+        return d;
+    }
+    __device__ __forceinline__ void advance() {
+        next += step;
+        left--;
+    }
+    __device__ __forceinline__ void fetch(int s) {
+        if (!kRing) return;
+        if (left > 0) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                if (whole(i))
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                     static_cast<uint32_t>(__cvta_generic_to_shared(slot(s, i)))), "l"(next + i * pitch)
+                                 : "memory");
+                else if (kShift && c0 + i * pitch + V > 0 && c0 + i * pitch < width)
+                    *slot(s, i) = edge(i);
+            }
+        } else {
+            clear(s);
+        }
+        advance();
+    }
+    __device__ __forceinline__ void read(int s, float (&v)[E]) {
         Pack<T, V> d[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int c = (i * tpr + t) * V - (kShift ? shift : 0);
-            if (r < rows && (kShift ? c + V > 0 && c < width : c < width)) {
-                if (kRing) d[i] = *slot(s, i);
-                else d[i] = *reinterpret_cast<const Pack<T, V> *>(row(r) + c);
+            if (kRing) {
+                d[i] = *slot(s, i);
+            } else if (left > 0 && whole(i)) {
+                d[i] = *reinterpret_cast<const Pack<T, V> *>(next + i * pitch);
             } else {
 #pragma unroll
                 for (int q = 0; q < V; q++) d[i].v[q] = from_f32<T>(0.0f);
             }
         }
+        if (!kRing) advance();
 #pragma unroll
         for (int e = 0; e < E; e++) v[e] = to_f32(d[e / V].v[e % V]);
+    }
+    // x - mu in the columns of the row, 0 elsewhere (where x reads as 0)
+    __device__ __forceinline__ void centre(float (&v)[E], float mu) const {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = c0 + i * pitch;
+            const float m = kShift ? (c + V > 0 && c < width ? mu : 0.0f) : (c < width ? mu : 0.0f);
+#pragma unroll
+            for (int q = 0; q < V; q++) v[i * V + q] -= m;
+            if (kShift && m != 0.0f && !whole(i)) {
+#pragma unroll
+                for (int q = 0; q < V; q++)
+                    if (c + q < 0 || c + q >= width) v[i * V + q] = 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T *row, const float (&v)[E]) const {      // row: at the first vector
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = c0 + i * pitch;
+            Pack<T, V> p;
+#pragma unroll
+            for (int q = 0; q < V; q++) p.v[q] = from_f32<T>(v[i * V + q]);
+            if (whole(i)) {
+                *reinterpret_cast<Pack<T, V> *>(row + i * pitch) = p;
+            } else if (kShift) {
+#pragma unroll
+                for (int q = 0; q < V; q++)
+                    if (c + q >= 0 && c + q < width) row[i * pitch + q] = p.v[q];
+            }
+        }
+    }
+    __device__ __forceinline__ void param(const void *p, int is_f32, float otherwise, float (&v)[E]) const {
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = otherwise;
+        if (!p) return;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int c = c0 + i * pitch;
+            if (!is_f32 && !kShift && whole(i) && (reinterpret_cast<uintptr_t>(p) & (V * sizeof(T) - 1)) == 0) {
+                const Pack<T, V> d = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(p) + c);
+#pragma unroll
+                for (int q = 0; q < V; q++) v[i * V + q] = to_f32(d.v[q]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < V; q++)
+                    if (c + q >= 0 && c + q < width) v[i * V + q] = param_at<T>(p, is_f32, c + q);
+            }
+        }
     }
 };
 
 __device__ __forceinline__ void fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void wait_row() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
-
-template <typename T, int V, int E, bool kShift>
-__device__ __forceinline__ void store_part(T *row, int width, int tpr, int t, int shift, const float (&v)[E]) {
-#pragma unroll
-    for (int i = 0; i < E / V; i++) {
-        const int c = (i * tpr + t) * V - (kShift ? shift : 0);
-        Pack<T, V> p;
-#pragma unroll
-        for (int q = 0; q < V; q++) p.v[q] = from_f32<T>(v[i * V + q]);
-        if (kShift ? c >= 0 && c + V <= width : c < width) {
-            *reinterpret_cast<Pack<T, V> *>(row + c) = p;
-        } else if (kShift) {
-#pragma unroll
-            for (int q = 0; q < V; q++)
-                if (c + q >= 0 && c + q < width) row[c + q] = p.v[q];
-        }
-    }
-}
-
-template <typename T, int V, int E>
-__device__ __forceinline__ void load_param(const void *p, int is_f32, float otherwise, int width, int tpr, int t, int shift,
-                                           float (&v)[E]) {
-#pragma unroll
-    for (int e = 0; e < E; e++) v[e] = otherwise;
-    if (!p) return;
-    if (is_f32) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int c = column<V>(e, tpr, t, shift);
-            if (c >= 0 && c < width) v[e] = static_cast<const float *>(p)[c];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int c = column<V>(e, tpr, t, shift);
-            if (c >= 0 && c < width) v[e] = to_f32(static_cast<const T *>(p)[c]);
-        }
-    }
-}
 
 // Elements between the 16-byte boundary below a row's address and the row.  The same for every row
 // of a group: the rows of a group lie a multiple of V rows apart.
@@ -210,46 +235,44 @@ __device__ __forceinline__ int row_shift(const void *base, int64_t row, int64_t 
     return (int)((reinterpret_cast<uintptr_t>(base) / sizeof(T) + (uint64_t)(row * stride)) & (V - 1));
 }
 
-template <typename T, int V, int E, bool kShift>
-__global__ void __launch_bounds__(kMaxTpr) forward_kernel(const Args a) {
+template <typename T, int V, int E, bool kShift, int B>
+__global__ void __launch_bounds__(B, B == kBlock ? 3 : 1) forward_kernel(const Args a) {
     __shared__ __align__(16) float red[2][1][16];
     extern __shared__ __align__(16) uint8_t ring[];
     int slot = 0;
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), groups = blockDim.x / tpr;
-    const int64_t first = (int64_t)blockIdx.x * groups + threadIdx.x / tpr, step = (int64_t)gridDim.x * groups;
+    const int64_t first = (int64_t)blockIdx.x * groups + threadIdx.x / tpr, every = (int64_t)gridDim.x * groups;
     const int shift = row_shift<T, V, kShift>(a.x, first, a.x_stride);
-    const Stream<T, V, E, kShift> x = {ring, (uint32_t)(E / V * blockDim.x * 16), static_cast<const T *>(a.x), a.x_stride,
-                                       a.rows, a.width, tpr, t, shift};
+    Stream<T, V, E, kShift> x(ring, E / V * blockDim.x * 16, a.x, first, every, a.x_stride, a, t, shift);
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
-        x.fetch(first + k * step, k);
+        x.fetch(k);
         fetched();
     }
     float w[E], b[E];
-    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, shift, w);
-    load_param<T, V, E>(a.b, a.param_f32, 0.0f, a.width, tpr, t, shift, b);
-    const uint32_t mine = columns_of<V, E>(a.width, tpr, t, shift);
+    x.param(a.w, a.param_f32, 1.0f, w);
+    x.param(a.b, a.param_f32, 0.0f, b);
     const float inv = 1.0f / (float)a.width;
+    T *y = static_cast<T *>(a.y) + first * a.width + x.c0;
     // every thread of a warp makes the same number of rounds: the sums are warp-wide
-    const int64_t rounds = (a.rows - (int64_t)blockIdx.x * groups + step - 1) / step;
+    const int rounds = (int)((a.rows - (int64_t)blockIdx.x * groups + every - 1) / every);
     int64_t r = first;
-    for (int64_t i = 0; i < rounds; i++, r += step) {
-        const int s = (int)(i % kStages);
+    int s = 0;
+    for (int i = 0; i < rounds; i++) {
         wait_row();
         float v[E];
-        x.read(r, s, v);
-        x.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
+        x.read(s, v);
+        x.fetch(s == 0 ? kAhead : s - 1);
         fetched();
+        s = s == kAhead ? 0 : s + 1;
         float m[1] = {0.0f}, q[1] = {0.0f};
 #pragma unroll
         for (int e = 0; e < E; e++) m[0] += v[e];
         group_sum<1>(m, tpr, red, slot);
         const float mu = m[0] * inv;
+        x.centre(v, mu);
 #pragma unroll
-        for (int e = 0; e < E; e++) {
-            v[e] = mine & (1u << (kShift ? e : e / V * V)) ? v[e] - mu : 0.0f;
-            q[0] += __fmul_rn(v[e], v[e]);
-        }
+        for (int e = 0; e < E; e++) q[0] += __fmul_rn(v[e], v[e]);
         group_sum<1>(q, tpr, red, slot);
         const float rstd = rsqrtf(q[0] * inv + a.eps);
         if (r < a.rows) {
@@ -259,73 +282,80 @@ __global__ void __launch_bounds__(kMaxTpr) forward_kernel(const Args a) {
             }
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = v[e] * rstd * w[e] + b[e];
-            store_part<T, V, E, kShift>(static_cast<T *>(a.y) + r * (int64_t)a.width, a.width, tpr, t, shift, v);
+            x.store(y, v);
         }
+        y += every * a.width;
+        r += every;
     }
 }
 
-template <typename T, int V, int E, bool kShift>
-__global__ void __launch_bounds__(kMaxTpr) backward_kernel(const Args a) {
+template <typename T, int V, int E, bool kShift, int B>
+__global__ void __launch_bounds__(B, B == kBlock ? 2 : 1) backward_kernel(const Args a) {
     __shared__ __align__(16) float red[2][2][16];
     extern __shared__ __align__(16) uint8_t ring[];      // the rings of x and g; at the end (2, width) sums
     int slot = 0;
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
-    const int64_t first = (int64_t)blockIdx.x * groups + group, step = (int64_t)gridDim.x * groups;
+    const int64_t first = (int64_t)blockIdx.x * groups + group, every = (int64_t)gridDim.x * groups;
     const int shift = row_shift<T, V, kShift>(a.x, first, a.x_stride);
     const uint32_t part = E / V * blockDim.x * 16;
-    const Stream<T, V, E, kShift> x = {ring, 2 * part, static_cast<const T *>(a.x), a.x_stride, a.rows, a.width, tpr, t, shift};
-    const Stream<T, V, E, kShift> g = {ring + part, 2 * part, static_cast<const T *>(a.g), a.g_stride, a.rows, a.width, tpr, t, shift};
+    Stream<T, V, E, kShift> x(ring, 2 * part, a.x, first, every, a.x_stride, a, t, shift);
+    Stream<T, V, E, kShift> g(ring + part, 2 * part, a.g, first, every, a.g_stride, a, t, shift);
 #pragma unroll
     for (int k = 0; k < kAhead; k++) {
-        x.fetch(first + k * step, k);
-        g.fetch(first + k * step, k);
+        x.fetch(k);
+        g.fetch(k);
         fetched();
     }
     float w[E], gw[E], gb[E];
-    load_param<T, V, E>(a.w, a.param_f32, 1.0f, a.width, tpr, t, shift, w);
-    const uint32_t mine = columns_of<V, E>(a.width, tpr, t, shift);
+    x.param(a.w, a.param_f32, 1.0f, w);
 #pragma unroll
     for (int e = 0; e < E; e++) gw[e] = gb[e] = 0.0f;
     const float inv = 1.0f / (float)a.width;
-    const int64_t rounds = (a.rows - (int64_t)blockIdx.x * groups + step - 1) / step;
+    T *gx = a.gx ? static_cast<T *>(a.gx) + first * a.width + x.c0 : nullptr;
+    const int rounds = (int)((a.rows - (int64_t)blockIdx.x * groups + every - 1) / every);
     int64_t r = first;
+    int s = 0;
     float mu_n = r < a.rows ? a.mean[r] : 0.0f, rstd_n = r < a.rows ? a.rstd[r] : 0.0f;
-    for (int64_t i = 0; i < rounds; i++, r += step) {
-        const int s = (int)(i % kStages);
+    for (int i = 0; i < rounds; i++) {
+        // (of a group without a row: the last row's, against a g of zeros)
         const float mu = mu_n, rstd = rstd_n;
-        if (r + step < a.rows) {
-            mu_n = a.mean[r + step];
-            rstd_n = a.rstd[r + step];
+        if (r + every < a.rows) {
+            mu_n = a.mean[r + every];
+            rstd_n = a.rstd[r + every];
         }
         wait_row();
         float u[E], v[E];
-        x.read(r, s, u);
-        g.read(r, s, v);
-        x.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
-        g.fetch(r + kAhead * step, (int)((i + kAhead) % kStages));
+        x.read(s, u);
+        g.read(s, v);
+        x.fetch(s == 0 ? kAhead : s - 1);
+        g.fetch(s == 0 ? kAhead : s - 1);
         fetched();
+        s = s == kAhead ? 0 : s + 1;
         float m[2] = {0.0f, 0.0f};
+        x.centre(u, r < a.rows ? mu : 0.0f);
 #pragma unroll
         for (int e = 0; e < E; e++) {
-            u[e] = mine & (1u << (kShift ? e : e / V * V)) ? (u[e] - mu) * rstd : 0.0f;
+            u[e] *= rstd;
             gw[e] += v[e] * u[e];
             gb[e] += v[e];
             v[e] *= w[e];
             m[0] += v[e];
             m[1] += __fmul_rn(v[e], u[e]);
         }
-        if (!a.gx) continue;
-        group_sum<2>(m, tpr, red, slot);
-        const float s1 = m[0] * inv, s2 = m[1] * inv;
-        if (r < a.rows) {
+        if (gx) {
+            group_sum<2>(m, tpr, red, slot);
+            const float s1 = m[0] * inv, s2 = m[1] * inv;
+            if (r < a.rows) {
 #pragma unroll
-            for (int e = 0; e < E; e++) u[e] = rstd * (v[e] - s1 - __fmul_rn(u[e], s2));
-            store_part<T, V, E, kShift>(static_cast<T *>(a.gx) + r * (int64_t)a.width, a.width, tpr, t, shift, u);
+                for (int e = 0; e < E; e++) u[e] = rstd * (v[e] - s1 - __fmul_rn(u[e], s2));
+                x.store(gx, u);
+            }
+            gx += every * a.width;
         }
+        r += every;
     }
     if (!a.partial) return;
-    // join the groups in their order; rows past the end added nothing (mu, rstd of a finished group are stale,
-    // its g is zero)
+    // join the groups in their order
     float *sums = reinterpret_cast<float *>(ring);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
@@ -333,7 +363,7 @@ __global__ void __launch_bounds__(kMaxTpr) backward_kernel(const Args a) {
         if (group == k) {
 #pragma unroll
             for (int e = 0; e < E; e++) {
-                const int c = column<V>(e, tpr, t, shift);
+                const int c = x.c0 + e / V * x.pitch + e % V;
                 if (c >= 0 && c < a.width) {
                     sums[c] = (k ? sums[c] : 0.0f) + gw[e];
                     sums[a.width + c] = (k ? sums[a.width + c] : 0.0f) + gb[e];
@@ -491,9 +521,10 @@ size_t ring_bytes(const Spread &s, size_t es) {
     return s.vec * es == 16 ? (size_t)kStages * (s.elems / s.vec) * s.threads * 16 : 0;
 }
 
-// Blocks that give every thread group rows a multiple of 8 apart (equal row shifts).
+// At most `most` blocks (one wave); a multiple of 8, which puts the rows of every thread group a multiple of
+// 8 apart (equal row shifts).
 int64_t blocks_of(int64_t rows, int groups, int64_t most) {
-    return (min64((rows + groups - 1) / groups, most) + 7) / 8 * 8;
+    return min64(((rows + groups - 1) / groups + 7) / 8 * 8, most / 8 * 8);
 }
 
 // Blocks of the backward: about one wave, so that the partial sums stay few.
@@ -546,7 +577,7 @@ extern "C" int feq_layer_norm_fwd(const void *x, int64_t rows, int64_t x_stride,
     const lnorm::Spread sp = lnorm::spread(at, width, es);
     a.tpr = sp.tpr;
     const int groups = sp.threads / sp.tpr;
-    const unsigned grid = (unsigned)lnorm::blocks_of(rows, groups, (int64_t)sm_count() * (1024 / sp.threads));
+    const unsigned grid = (unsigned)lnorm::blocks_of(rows, groups, (int64_t)sm_count() * (768 / sp.threads));
     const size_t smem = lnorm::ring_bytes(sp, es);
     auto go = [&](auto kern) -> int {
         if (smem > 48 * 1024 - 1024)
@@ -559,10 +590,13 @@ extern "C" int feq_layer_norm_fwd(const void *x, int64_t rows, int64_t x_stride,
     FEQ_TOKEN_TYPE(dtype, {
         constexpr int W = 16 / sizeof(T);
         if (sp.shift) {
-            rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, W, 8, true> : lnorm::forward_kernel<T, W, 16, true>);
+            rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, W, 8, true, 256>
+                    : sp.threads == 256 ? lnorm::forward_kernel<T, W, 16, true, 256> : lnorm::forward_kernel<T, W, 16, true, 512>);
         } else {
             FEQ_TOKEN_VEC(T, sp.vec, {
-                rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, V, 8, false> : lnorm::forward_kernel<T, V, 16, false>);
+                rc = go(sp.elems == 8 ? lnorm::forward_kernel<T, V, 8, false, 256>
+                        : sp.threads == 256 ? lnorm::forward_kernel<T, V, 16, false, 256>
+                                            : lnorm::forward_kernel<T, V, 16, false, 512>);
             })
         }
     })
@@ -633,10 +667,13 @@ extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, con
         FEQ_TOKEN_TYPE(dtype, {
             constexpr int W = 16 / sizeof(T);
             if (sp.shift) {
-                rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, W, 8, true> : lnorm::backward_kernel<T, W, 16, true>);
+                rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, W, 8, true, 256>
+                    : sp.threads == 256 ? lnorm::backward_kernel<T, W, 16, true, 256> : lnorm::backward_kernel<T, W, 16, true, 512>);
             } else {
                 FEQ_TOKEN_VEC(T, sp.vec, {
-                    rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, V, 8, false> : lnorm::backward_kernel<T, V, 16, false>);
+                    rc = go(sp.elems == 8 ? lnorm::backward_kernel<T, V, 8, false, 256>
+                        : sp.threads == 256 ? lnorm::backward_kernel<T, V, 16, false, 256>
+                                            : lnorm::backward_kernel<T, V, 16, false, 512>);
                 })
             }
         })

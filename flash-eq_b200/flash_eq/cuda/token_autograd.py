@@ -19,26 +19,28 @@ from . import token_ops
 
 
 def _tracks(*tensors) -> bool:
-    if not torch.is_grad_enabled():
-        return False
-    return any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = token_ops.layer_norm_fwd(x, weight, bias, eps, keep_stats=True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = token_ops.layer_norm_fwd(x, weight, bias, eps, keep_stats=True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.param_dtype = next((p.dtype for p in (weight, bias) if p is not None), None)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        return (*token_ops.layer_norm_bwd(grad_out, x, weight, mean, rstd, need[0], need[1], need[2],
-                                          ctx.param_dtype), None)
+        return (*token_ops.layer_norm_bwd(grad_out, x, weight, stats, need[0], need[1], need[2], ctx.param_dtype),
+                None)
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,

@@ -21,31 +21,35 @@ MAX_EXPERTS, MAX_TOP_K = 512, 32
 
 # These wrappers run in front of kernels of a few microseconds, so they pass plain integers to ctypes and
 # ask torch for a stream handle without building a Stream object.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # absent in builds without CUDA
+_current_device = torch.cuda.current_device
+_empty, _f32, _i32 = torch.empty, torch.float32, torch.int32
+_load = _lib.load
 
 
 def _ready(first: torch.Tensor, *others):
     """The library, after checking that every tensor lies on one CUDA device."""
     dev = first.get_device()
-    if dev < 0 or any(t is not None and t.get_device() != dev for t in others):
+    good = dev >= 0
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            good = False
+    if not good:
         _require_cuda(first, *others)
         raise RuntimeError("flash-eq ops need all tensors on one device; got "
                            + ", ".join(str(t.device) for t in (first, *others) if t is not None))
-    return _lib.load()
+    return _load()
 
 
 def _call(fn, what: str, dev: int, *args) -> None:
     """fn(*args, stream) with ``dev`` current, on its current stream."""
-    rc = _call_rc(fn, dev, *args)
+    if dev == _current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
-
-
-def _call_rc(fn, dev: int, *args) -> int:
-    if dev == torch.cuda.current_device():
-        return fn(*args, _raw_stream(dev))
-    with torch.cuda.device(dev):
-        return fn(*args, _raw_stream(dev))
 
 
 def _ptr(t) -> int | None:
@@ -67,7 +71,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _param(p, like: torch.Tensor, width: int, name: str):
     if p is None:
         return None
-    if p.dim() != 1 or p.shape[0] != width:
+    if p.shape != (width,):
         raise ValueError(f"{name} must have shape ({width},); got {tuple(p.shape)}")
     if p.dtype is not like.dtype and p.dtype is not torch.float32:
         raise TypeError(f"{name} must be {like.dtype} or float32; got {p.dtype}")
@@ -75,14 +79,14 @@ def _param(p, like: torch.Tensor, width: int, name: str):
 
 
 def _workspace(nbytes: int, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return _empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 # ---------------------------------------------------------------------------
 # layer norm
 # ---------------------------------------------------------------------------
 def layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, keep_stats: bool):
-    """(y, mean, rstd) of x (..., D); mean / rstd None unless ``keep_stats``."""
+    """(y, stats) of x (..., D); stats (2, rows) = mean and 1 / std, None unless ``keep_stats``."""
     lib = _ready(x, weight, bias)
     code = _dtype(x, "x")
     width = x.shape[-1] if x.dim() else 0
@@ -96,19 +100,20 @@ def layer_norm_fwd(x: torch.Tensor, weight, bias, eps: float, keep_stats: bool):
         raise TypeError(f"weight and bias must have one type; got {weight.dtype} and {bias.dtype}")
     rows = _rows(x if x.dim() == 2 else x.reshape(-1, width))
     n, dev = rows.shape[0], x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean = rstd = None
+    y = _empty(x.shape, dtype=x.dtype, device=dev)
+    stats = mean = rstd = None
     if keep_stats:
-        mean = torch.empty(n, dtype=torch.float32, device=dev)
-        rstd = torch.empty(n, dtype=torch.float32, device=dev)
+        stats = _empty(2, n, dtype=_f32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
     p = bias if weight is None else weight
     _call(lib.feq_layer_norm_fwd, "feq_layer_norm_fwd", dev.index, rows.data_ptr(), n, rows.stride(0), width, code,
-          _ptr(weight), _ptr(bias), int(p is not None and p.dtype is torch.float32), eps, y.data_ptr(), _ptr(mean),
-          _ptr(rstd))
-    return y, mean, rstd
+          None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+          p is not None and p.dtype is _f32, eps, y.data_ptr(), mean, rstd)
+    return y, stats
 
 
-def layer_norm_bwd(grad_out, x, weight, mean, rstd, need_x=True, need_weight=True, need_bias=True, param_dtype=None):
+def layer_norm_bwd(grad_out, x, weight, stats, need_x=True, need_weight=True, need_bias=True, param_dtype=None):
     """(grad_x, grad_weight, grad_bias) of ``layer_norm_fwd``; None where not needed."""
     lib = _ready(grad_out, x, weight)
     code, width = _dtype(x, "x"), x.shape[-1]
@@ -116,14 +121,15 @@ def layer_norm_bwd(grad_out, x, weight, mean, rstd, need_x=True, need_weight=Tru
     rows, g = _rows(x.reshape(-1, width)), _rows(grad_out.reshape(-1, width))
     n, dev = rows.shape[0], x.device
     pd = param_dtype or (weight.dtype if weight is not None else x.dtype)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    gw = torch.empty(width, dtype=pd, device=dev) if need_weight else None
-    gb = torch.empty(width, dtype=pd, device=dev) if need_bias else None
+    gx = _empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    gw = _empty(width, dtype=pd, device=dev) if need_weight else None
+    gb = _empty(width, dtype=pd, device=dev) if need_bias else None
+    mean = stats.data_ptr()
     nbytes = lib.feq_layer_norm_bwd_workspace_bytes(n, width) if need_weight or need_bias else 0
     ws = _workspace(nbytes, dev)
     _call(lib.feq_layer_norm_bwd, "feq_layer_norm_bwd", dev.index, g.data_ptr(), g.stride(0), rows.data_ptr(), n,
-          rows.stride(0), width, code, _ptr(weight), int(pd is torch.float32), mean.data_ptr(), rstd.data_ptr(),
-          _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), nbytes)
+          rows.stride(0), width, code, _ptr(weight), pd is _f32, mean, mean + 4 * n, _ptr(gx), _ptr(gw),
+          _ptr(gb), _ptr(ws), nbytes)
     return gx, gw, gb
 
 
@@ -143,14 +149,14 @@ def expert_route(logits: torch.Tensor, top_k: int, normalize: bool = True):
     if e > MAX_EXPERTS or k > MAX_TOP_K:
         raise ValueError(f"at most {MAX_EXPERTS} experts and top_k {MAX_TOP_K}; got {e} and {k}")
     rows, dev = _rows(logits), logits.device
-    ids = torch.empty(n, k, dtype=torch.int32, device=dev)
-    slots = torch.empty(n, k, dtype=torch.int32, device=dev)
-    weights = torch.empty(n, k, dtype=torch.float32, device=dev)
-    offsets = torch.empty(e + 1, dtype=torch.int32, device=dev)
+    ids = _empty(n, k, dtype=_i32, device=dev)
+    slots = torch.empty_like(ids)
+    weights = _empty(n, k, dtype=_f32, device=dev)
+    offsets = _empty(e + 1, dtype=_i32, device=dev)
     nbytes = lib.feq_expert_route_workspace_bytes(n, k, e)
     ws = _workspace(nbytes, dev)
     _call(lib.feq_expert_route, "feq_expert_route", dev.index, rows.data_ptr(), n, rows.stride(0), e, k, code,
-          int(bool(normalize)), ids.data_ptr(), weights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), _ptr(ws),
+          bool(normalize), ids.data_ptr(), weights.data_ptr(), slots.data_ptr(), offsets.data_ptr(), _ptr(ws),
           nbytes)
     return ids, weights, slots, offsets
 
@@ -160,9 +166,9 @@ def expert_route_bwd(logits, ids, weights, grad_weights, normalize):
     n, e = logits.shape
     rows, dev = _rows(logits), logits.device
     grad_weights = grad_weights.to(torch.float32).contiguous()
-    out = torch.empty(n, e, dtype=logits.dtype, device=dev)
+    out = _empty(n, e, dtype=logits.dtype, device=dev)
     _call(lib.feq_expert_route_bwd, "feq_expert_route_bwd", dev.index, rows.data_ptr(), n, rows.stride(0), e,
-          ids.shape[1], _dtype(logits, "logits"), int(bool(normalize)), ids.data_ptr(), weights.data_ptr(),
+          ids.shape[1], _dtype(logits, "logits"), bool(normalize), ids.data_ptr(), weights.data_ptr(),
           grad_weights.data_ptr(), out.data_ptr())
     return out
 
@@ -182,7 +188,7 @@ def expert_dispatch(x: torch.Tensor, slots, offsets) -> torch.Tensor:
     if x.dim() != 2 or x.shape[0] != n or x.shape[1] < 1:
         raise ValueError(f"x must be ({n}, width); got {tuple(x.shape)}")
     code, rows, width = _dtype(x, "x"), _rows(x), x.shape[1]
-    out = torch.empty(n * k, width, dtype=x.dtype, device=x.device)
+    out = _empty(n * k, width, dtype=x.dtype, device=x.device)
     _call(lib.feq_expert_dispatch, "feq_expert_dispatch", x.device.index, rows.data_ptr(), n, rows.stride(0), width,
           code, k, e, slots.data_ptr(), offsets.data_ptr(), out.data_ptr())
     return out
@@ -203,7 +209,7 @@ def expert_combine(y: torch.Tensor, slots, offsets, weights=None) -> torch.Tenso
         if weights.shape != slots.shape or weights.dtype is not torch.float32:
             raise ValueError(f"weights must be a float32 ({n}, {k}) tensor; got {weights.dtype} {tuple(weights.shape)}")
         weights = weights.contiguous()
-    out = torch.empty(n, width, dtype=y.dtype, device=y.device)
+    out = _empty(n, width, dtype=y.dtype, device=y.device)
     _call(lib.feq_expert_combine, "feq_expert_combine", y.device.index, rows.data_ptr(), rows.stride(0), n, width,
           code, k, e, slots.data_ptr(), offsets.data_ptr(), _ptr(weights), out.data_ptr())
     return out
@@ -214,8 +220,8 @@ def expert_combine_bwd(grad_out, y, slots, offsets, weights):
     lib = _ready(grad_out, y, slots, offsets, weights)
     n, k, e = _plan(slots, offsets)
     code, rows, g, width = _dtype(y, "y"), _sorted_rows(y, n, k), _rows(grad_out), y.shape[1]
-    gy = torch.empty(n * k, width, dtype=y.dtype, device=y.device)
-    gw = torch.empty(n, k, dtype=torch.float32, device=y.device)
+    gy = _empty(n * k, width, dtype=y.dtype, device=y.device)
+    gw = _empty(n, k, dtype=_f32, device=y.device)
     weights = weights.contiguous()
     _call(lib.feq_expert_combine_bwd, "feq_expert_combine_bwd", y.device.index, g.data_ptr(), g.stride(0),
           rows.data_ptr(), rows.stride(0), n, width, code, k, e, slots.data_ptr(), offsets.data_ptr(),
@@ -274,12 +280,15 @@ def _linear_args(x, weight, offsets, lvals):
 def _run_linear(lib, fn, what, a, backward, device, status):
     if status is not None:
         a.status = status.data_ptr()
-    ref = ctypes.byref(a)
-    rc = _call_rc(fn, device.index, ref, None, 0)
+    ref, dev = ctypes.byref(a), device.index
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return _run_linear(lib, fn, what, a, backward, device, None)
+    rc = fn(ref, None, 0, _raw_stream(dev))
     if rc == _lib.FEQ_ERR_WORKSPACE:          # an operand has to be packed, or sums joined
         nbytes = lib.feq_expert_linear_workspace_bytes(ref, backward)
         ws = _workspace(nbytes, device)
-        rc = _call_rc(fn, device.index, ref, _ptr(ws), nbytes)
+        rc = fn(ref, ws.data_ptr(), nbytes, _raw_stream(dev))
     if rc:
         _lib.check(rc, what)
 
@@ -298,7 +307,7 @@ def expert_linear_fwd(x, weight, bias, offsets, lvals, status=None) -> torch.Ten
             raise TypeError(f"bias must have x's type {x.dtype}; got {bias.dtype}")
         bias = bias.contiguous()
         a.bias = bias.data_ptr()
-    out = torch.empty((x.shape[0], a.c_out) if plain else (x.shape[0], x.shape[1], a.c_out), dtype=x.dtype,
+    out = _empty((x.shape[0], a.c_out) if plain else (x.shape[0], x.shape[1], a.c_out), dtype=x.dtype,
                       device=x.device)
     a.out = out.data_ptr()
     _run_linear(lib, lib.feq_expert_linear_fwd, "feq_expert_linear_fwd", a, 0, x.device, status)
@@ -310,11 +319,11 @@ def expert_linear_bwd(grad_out, x, weight, offsets, lvals, need_x=True, need_wei
     lib = _ready(grad_out, x, weight, offsets)
     a, kept, scalars = _linear_args(x, weight, offsets, lvals)
     g, dev, plain = _strided(grad_out), x.device, x.dim() == 2
-    gx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    gw = torch.empty(weight.shape, dtype=x.dtype, device=dev) if need_weight else None
+    gx = _empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    gw = _empty(weight.shape, dtype=x.dtype, device=dev) if need_weight else None
     gb = None
     if need_bias:
-        gb = torch.empty((a.num_experts, a.c_out) if plain else (a.num_experts, scalars, a.c_out), dtype=x.dtype,
+        gb = _empty((a.num_experts, a.c_out) if plain else (a.num_experts, scalars, a.c_out), dtype=x.dtype,
                          device=dev)
     a.grad_out, a.grad_row_stride, a.grad_comp_stride = g.data_ptr(), g.stride(0), 0 if plain else g.stride(1)
     a.grad_x, a.grad_weight, a.grad_bias = _ptr(gx), _ptr(gw), _ptr(gb)
