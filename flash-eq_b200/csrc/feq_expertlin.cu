@@ -519,52 +519,87 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
     if (threadIdx.x == 0 && abort_s) set_status(a.status, 2);
 }
 
-// gW = the sum of an expert's partial sums, in their order.
-template <typename T>
+// An expert's partial sums added up in their order: parts of chunk_rows rows, `per` vectors of `size`
+// values each (the irreps of gW, the scalars of gb).
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
-join_kernel(const float *__restrict__ part, const int32_t *offsets, int experts, int64_t rows, int chunk_rows, int reps,
+join_kernel(const float *__restrict__ part, const int32_t *offsets, int experts, int64_t rows, int chunk_rows, int per,
             int64_t size, T *__restrict__ out) {
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     lay_out(offsets, experts, rows, off, pre, [&](int32_t n) { return (n + chunk_rows - 1) / chunk_rows; });
-    const int e = blockIdx.y / reps, rep = blockIdx.y % reps;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-        float s = 0.0f;
-        for (int u = pre[e]; u < pre[e + 1]; u++) s += part[((int64_t)u * reps + rep) * size + i];
-        out[(int64_t)blockIdx.y * size + i] = from_f32<T>(s);
+    const int e = blockIdx.x / per, k = blockIdx.x % per;
+    for (int64_t i = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.y * 256 * V) {
+        float s[V];
+#pragma unroll
+        for (int q = 0; q < V; q++) s[q] = 0.0f;
+#pragma unroll 4
+        for (int u = pre[e]; u < pre[e + 1]; u++) {
+            const Pack<float, V> d = *reinterpret_cast<const Pack<float, V> *>(part + ((int64_t)u * per + k) * size + i);
+#pragma unroll
+            for (int q = 0; q < V; q++) s[q] += d.v[q];
+        }
+        Pack<T, V> o;
+#pragma unroll
+        for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(s[q]);
+        *reinterpret_cast<Pack<T, V> *>(out + (int64_t)blockIdx.x * size + i) = o;
     }
 }
 
-// gb of one expert and scalar: 32 columns a block, a warp per 32nd row, sums joined in warp order.
-template <typename T>
-__global__ void __launch_bounds__(1024)
-bias_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const int32_t *offsets, int experts, int64_t rows,
-            int cout, const __grid_constant__ Comps c, T *__restrict__ out) {
+// gb, step 1: the columns of one part of an expert's rows (kBiasRows of them) and one scalar.  A warp
+// reads V channels a lane of every 8th row; the warps' sums are joined in their order.
+constexpr int kBiasRows = 256;
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+bias_part_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const int32_t *offsets, int experts, int64_t rows,
+                 int cout, const __grid_constant__ Comps c, float *__restrict__ part) {
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
-    __shared__ float sh[32][33];
-    lay_out(offsets, experts, rows, off, pre, [](int32_t) { return 0; });
-    const int e = blockIdx.y / c.scalars, sc = blockIdx.y % c.scalars;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, o = blockIdx.x * 32 + lane;
+    __shared__ float sh[8][32 * V + 1];
+    lay_out(offsets, experts, rows, off, pre, [](int32_t n) { return (n + kBiasRows - 1) / kBiasRows; });
+    const int unit = blockIdx.x / c.scalars, sc = blockIdx.x % c.scalars;
+    if (unit >= pre[experts]) return;
+    int lo = 0, hi = experts;                 // the expert of this unit: pre[lo] <= unit < pre[lo + 1]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (pre[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    while (pre[lo + 1] <= unit) lo++;
+    const int64_t r0 = off[lo] + (int64_t)(unit - pre[lo]) * kBiasRows, r1 = min64(r0 + kBiasRows, off[lo + 1]);
     int rep = 0;
     while (c.scalar_of[rep] != sc) rep++;
-    const T *col = g + c.first[rep] * g_comp + o;
-    float s = 0.0f;
-    if (o < cout)
-        for (int64_t r = off[e] + warp; r < off[e + 1]; r += 32) s += to_f32(col[r * g_row]);
-    sh[warp][lane] = s;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, o = (blockIdx.y * 32 + lane) * V;
+    float s[V];
+#pragma unroll
+    for (int q = 0; q < V; q++) s[q] = 0.0f;
+    if (o < cout) {
+        const T *col = g + c.first[rep] * g_comp + o;
+#pragma unroll 8
+        for (int64_t r = r0 + warp; r < r1; r += 8) {
+            const Pack<T, V> d = *reinterpret_cast<const Pack<T, V> *>(col + r * g_row);
+#pragma unroll
+            for (int q = 0; q < V; q++) s[q] += to_f32(d.v[q]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < V; q++) sh[warp][lane * V + q] = s[q];
     __syncthreads();
-    if (warp == 0 && o < cout) {
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int col = blockIdx.y * 32 * V + i;
+        if (col >= cout) break;
         float v = 0.0f;
-        for (int k = 0; k < 32; k++) v += sh[k][lane];
-        out[(int64_t)blockIdx.y * cout + o] = from_f32<T>(v);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v += sh[k][i];
+        part[((int64_t)unit * c.scalars + sc) * cout + col] = v;
     }
 }
 
 // Rows (rows, dim, n) with strides of their own -> planes (PLANES, rows, dim, npad) of 16-bit values,
-// zeros from n to npad (a multiple of 8).  PLANES 3: float32 as three bfloat16 summing to it.
+// zeros from n to npad (a multiple of 8).  PLANES 3: float32 as three bfloat16 summing to it.  With
+// `reps` > 0 the rows are weights, reps per expert, and experts without rows of their own are left out.
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
 pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, int64_t row, int64_t comp,
-            uint16_t *__restrict__ dst) {
+            uint16_t *__restrict__ dst, int reps, const int32_t *__restrict__ offsets) {
     const int units = npad / 8;
     const int64_t total = rows * dim * units, plane = rows * dim * (int64_t)npad;
     const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uint64_t)row * sizeof(T) | (uint64_t)comp * sizeof(T)) & 15) == 0;
@@ -572,6 +607,7 @@ pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, i
         const int64_t rd = i / units;
         const int k0 = (int)(i - rd * units) * 8;
         const int64_t r = dim == 1 ? rd : rd / dim;
+        if (reps > 0 && offsets[r / reps + 1] <= offsets[r / reps]) continue;
         const T *s = src + r * row + (rd - r * dim) * comp + k0;
         T v[8];
         if (wide && k0 + 8 <= n) {
@@ -676,7 +712,7 @@ static size_t packed_bytes(int dtype, int64_t rows, int dim, int n) {
 
 // The operand as the kernels read it: where it lies, or packed into the workspace.
 static int operand(Operand *o, const void *p, int dtype, int64_t rows, int dim, int n, int64_t row, int64_t comp,
-                   WsCarver *ws, cudaStream_t s) {
+                   WsCarver *ws, cudaStream_t s, int reps = 0, const int32_t *offsets = nullptr) {
     o->rows = rows;
     o->dim = dim;
     o->n = n;
@@ -694,9 +730,11 @@ static int operand(Operand *o, const void *p, int dtype, int64_t rows, int dim, 
     const unsigned grid = (unsigned)max64(1, min64((rows * dim * (np / 8) + 255) / 256, (int64_t)sm_count() * 16));
     uint16_t *d = static_cast<uint16_t *>(dst);
     if (dtype == FEQ_DTYPE_F32)
-        pack_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float *>(p), rows, dim, n, np, row, comp, d);
+        pack_kernel<float, 3><<<grid, 256, 0, s>>>(static_cast<const float *>(p), rows, dim, n, np, row, comp, d,
+                                                  reps, offsets);
     else
-        pack_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16 *>(p), rows, dim, n, np, row, comp, d);
+        pack_kernel<__nv_bfloat16, 1><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16 *>(p), rows, dim, n, np, row, comp,
+                                                          d, reps, offsets);
     FEQ_LAUNCH_CHECK();
     o->base = dst;
     o->comp = np;
@@ -815,6 +853,8 @@ static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool 
         const int part = part_rows(q, c, grad_w_width(q));
         if (part > 0) ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
     }
+    if (backward && q.grad_bias && c.scalars)
+        ws.take((size_t)(q.rows / kBiasRows + min64(q.num_experts, q.rows)) * c.scalars * q.c_out * sizeof(float));
     return (ws.used + 255) & ~size_t(255);       // in any order of the regions
 }
 
@@ -843,6 +883,18 @@ static Params params(const FeqExpertLinearArgs &q) {
     a.status = q.status;
     a.wait_ns = wait_limit_ns();
     return a;
+}
+
+static int join(const float *part, const FeqExpertLinearArgs &q, const Comps &c, int chunk_rows, int per, int64_t size,
+                void *out, cudaStream_t s) {
+    const bool four = size % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const dim3 grid((unsigned)(q.num_experts * per), (unsigned)min64((size / (four ? 4 : 1) + 255) / 256, 1024));
+    FEQ_TOKEN_TYPE(q.dtype, {
+        auto kern = four ? join_kernel<T, 4> : join_kernel<T, 1>;
+        kern<<<grid, 256, 0, s>>>(part, q.offsets, q.num_experts, q.rows, chunk_rows, per, size, static_cast<T *>(out));
+    })
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
 }
 
 // y or gx: rows A (rows, dim, K) times the weights.
@@ -880,7 +932,7 @@ extern "C" int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *work
     rc = elin::operand(&x, q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride, &ws, s);
     if (rc == FEQ_OK)
         rc = elin::operand(&w, q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in,
-                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s);
+                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s, c.reps, q.offsets);
     if (rc != FEQ_OK) return rc;
     return elin::row_product<elin::kForward>(q, c, x, w, q.out, s);
 }
@@ -910,7 +962,7 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
     }
     if (q.grad_x) {
         rc = elin::operand(&w, q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in,
-                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s);
+                           (int64_t)q.c_out * q.c_in, q.c_in, &ws, s, c.reps, q.offsets);
         if (rc == FEQ_OK) rc = elin::row_product<elin::kGradX>(q, c, g, w, q.grad_x, s);
         if (rc != FEQ_OK) return rc;
     }
@@ -935,20 +987,27 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
         rc = elin::run<elin::kGradW>(g, x, a, c, bn, tiles, s);
         if (rc != FEQ_OK) return rc;
         if (a.split) {
-            const int64_t size = (int64_t)q.c_in * q.c_out;
-            const dim3 grid((unsigned)min64((size + 255) / 256, 64), (unsigned)(q.num_experts * c.reps));
-            FEQ_TOKEN_TYPE(q.dtype, elin::join_kernel<T><<<grid, 256, 0, s>>>(
-                                        static_cast<const float *>(a.out), q.offsets, q.num_experts, q.rows, part, c.reps,
-                                        size, static_cast<T *>(q.grad_weight));)
-            FEQ_LAUNCH_CHECK();
+            rc = elin::join(static_cast<const float *>(a.out), q, c, part, c.reps, (int64_t)q.c_in * q.c_out,
+                            q.grad_weight, s);
+            if (rc != FEQ_OK) return rc;
         }
     }
     if (q.grad_bias && c.scalars) {
-        const dim3 grid((q.c_out + 31) / 32, q.num_experts * c.scalars);
-        FEQ_TOKEN_TYPE(q.dtype, elin::bias_kernel<T><<<grid, 1024, 0, s>>>(
-                                    static_cast<const T *>(q.grad_out), q.grad_row_stride, q.grad_comp_stride, q.offsets,
-                                    q.num_experts, q.rows, q.c_out, c, static_cast<T *>(q.grad_bias));)
+        const int64_t units = q.rows / elin::kBiasRows + min64(q.num_experts, q.rows);
+        float *part = static_cast<float *>(ws.take((size_t)units * c.scalars * q.c_out * sizeof(float)));
+        if (ws.used > ws.cap) return FEQ_ERR_WORKSPACE;
+        const int vec = vector_elems((uint64_t)(uintptr_t)q.grad_out | (uint64_t)q.grad_row_stride * es |
+                                         (uint64_t)q.grad_comp_stride * es | (uint64_t)q.c_out * es, es);
+        const unsigned gx = (unsigned)(units * c.scalars);
+        FEQ_TOKEN_TYPE(q.dtype, FEQ_TOKEN_VEC(T, vec, {
+            const dim3 grid(gx, (unsigned)((q.c_out + 32 * V - 1) / (32 * V)));
+            elin::bias_part_kernel<T, V><<<grid, 256, 0, s>>>(static_cast<const T *>(q.grad_out), q.grad_row_stride,
+                                                              q.grad_comp_stride, q.offsets, q.num_experts, q.rows,
+                                                              q.c_out, c, part);
+        }))
         FEQ_LAUNCH_CHECK();
+        rc = elin::join(part, q, c, elin::kBiasRows, c.scalars, q.c_out, q.grad_bias, s);
+        if (rc != FEQ_OK) return rc;
     }
     return FEQ_OK;
 }
