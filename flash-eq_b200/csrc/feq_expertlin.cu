@@ -13,11 +13,13 @@
 //   warp 1      one thread issues tcgen05.mma kind::f16 into one of two TMEM accumulators
 //   warps 2..5  epilogue: tcgen05.ld, + bias, through shared memory to row-contiguous stores, while
 //               the next tile's products run
-//   warp 6      (gW only) passes every chunk on to warp 1, and in the last chunk of an expert's rows
-//               first zeroes the rows that belong to the next expert, in both operands
+// Large 16-bit products run on pairs of CTAs (cta_group::2, 256 x 256 tiles): each CTA loads its 128 rows
+// of A and half of B's, which takes a third off the traffic through shared memory (writes plus reads,
+// 24 -> 16 KB per 16 of K and 128 cycles, of the 128 B a cycle that it moves): MEASURE_PAIR
 // The contraction runs over channels in y and gx and over rows in gW; an operand whose channels
 // are not the contraction is read MN-major (the shared-memory tile as the copy leaves it), so
-// nothing is transposed.  bfloat16 and float16 operands are read where they lie when a tensor
+// nothing is transposed; the last rows of an expert, where a chunk of 64 would reach into the next
+// expert's, come from a copy padded with zeros (tails_kernel).  bfloat16 and float16 operands are read where they lie when a tensor
 // map can describe them (16-byte addresses and strides), else from a packed copy.  float32: each
 // operand is packed as three bfloat16 planes whose sum is the value to 24 bits, and six products
 // (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave an error of 2^-24 of the terms; an infinite
@@ -26,6 +28,8 @@
 // its own (the five others add to a sum 2^-8 as large), and after kSegment chunks the epilogue
 // adds both to float32 registers (measured against float64 at K = 576: 3.9e-6 with one accumulator).
 #include <cuda.h>
+
+#include <stdio.h>
 
 #include <algorithm>
 
@@ -40,7 +44,7 @@ using namespace sm100;
 
 constexpr int kMaxExperts = 512;
 constexpr int BM = 128, BK = 64;
-constexpr int kThreads = 7 * 32;
+constexpr int kThreads = 6 * 32;
 constexpr uint32_t kBox = 64 * 128;                 // bytes of a 64-row, 64-channel box
 constexpr int kMaxStages = 8;
 constexpr int kSegment = 4;                         // chunks a float32 accumulator runs over
@@ -87,11 +91,111 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
     return d;
 }
 
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+// One box into this CTA's shared memory, counted on `bar` (a shared::cluster address; kPair: the first
+// CTA's barrier).
+template <bool kPair>
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    if (!kPair)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+            ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+            "[%0], [%1, {%2, %3, %4, %5}], [%6];"
+            ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+            : "memory");
+}
+
+// ---- two CTAs of a cluster working on one tile (cta_group::2) ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Address of `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t smem_at(const void *p, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t at) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(at) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    if (!kPair) return mbar_try_wait(bar, parity);
+    uint32_t ok;
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
         : "memory");
+    return ok != 0;
+}
+// Bounded wait; pairs acquire what the other CTA released.
+template <bool kPair>
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit_ns) {
+    const uint32_t b = smem_u32(bar);
+    if (try_wait<kPair>(b, parity)) return true;
+    const uint64_t t0 = globaltimer();
+    for (uint32_t i = 1;; i++) {
+        if (try_wait<kPair>(b, parity)) return true;
+        if ((i & 7) == 0) {
+            if (*abort_flag) return false;
+            if (globaltimer() - t0 > limit_ns) {
+                *abort_flag = 1;
+                return false;
+            }
+        }
+    }
+}
+template <bool kPair>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if (!kPair) {
+        umma_f16(d, a, b, idesc, accumulate);
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+// Arrive on `bar` (pair: of both CTAs) once every product issued so far is done.
+template <bool kPair>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    if (!kPair)
+        umma_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+            ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void tmem_take(uint32_t *dst, uint32_t cols) {
+    if (!kPair) {
+        tmem_alloc(dst, cols);
+        tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <bool kPair>
+__device__ __forceinline__ void tmem_give(uint32_t addr, uint32_t cols) {
+    if (!kPair)
+        tmem_dealloc(addr, cols);
+    else
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
 }
 
 // off[e] (never decreasing, within the rows) and pre[e] = first unit of expert e, where an expert
@@ -141,8 +245,9 @@ struct Tile {
     int part;                // gW: index of the partial sum
 };
 
-template <int MODE, int BN>
+template <int MODE, int BN, bool kPair>
 struct Walk {
+    static constexpr int kRows = kPair ? 2 * BM : BM;      // rows of a tile
     const Params &a;
     const Comps &c;
     const int32_t *off, *pre;
@@ -151,19 +256,19 @@ struct Walk {
     __device__ Walk(const Params &a_, const Comps &c_, const int32_t *off_, const int32_t *pre_)
         : a(a_), c(c_), off(off_), pre(pre_) {
         tiles_n = ((MODE == kGradW ? a.K : a.J) + BN - 1) / BN;
-        tiles_m = MODE == kGradW ? (a.J + BM - 1) / BM : 1;
+        tiles_m = MODE == kGradW ? (a.J + kRows - 1) / kRows : 1;
         total = (int64_t)pre[a.experts] * (MODE == kGradW ? c.reps * tiles_m : c.dim) * tiles_n;
-        t = blockIdx.x;
+        t = blockIdx.x / (kPair ? 2 : 1);
     }
     __device__ bool next(Tile &q) {
         if (t >= total) return false;
         int64_t u = t;
-        t += gridDim.x;
+        t += gridDim.x / (kPair ? 2 : 1);
         const int nt = (int)(u % tiles_n);
         u /= tiles_n;
         q.n0 = nt * BN;
         if (MODE == kGradW) {
-            q.m0 = (int)(u % tiles_m) * BM;
+            q.m0 = (int)(u % tiles_m) * kRows;
             u /= tiles_m;
         } else {
             q.m0 = 0;
@@ -173,7 +278,7 @@ struct Walk {
         const int unit = (int)(u / inner);
         while (pre[e + 1] <= unit) e++;
         q.e = e;
-        const int span = MODE == kGradW ? a.chunk_rows : BM;
+        const int span = MODE == kGradW ? a.chunk_rows : kRows;
         q.r0 = off[e] + (int64_t)(unit - pre[e]) * span;
         q.r1 = min64(q.r0 + span, off[e + 1]);
         q.part = unit * c.reps + q.p;
@@ -185,33 +290,36 @@ struct Walk {
     }
 };
 
-template <int MODE, int PLANES, int BN>
+template <int MODE, int PLANES, int BN, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+            const __grid_constant__ CUtensorMap atail, const __grid_constant__ CUtensorMap btail,
             const __grid_constant__ Params a, const __grid_constant__ Comps c) {
     constexpr bool kAmn = MODE == kGradW, kBmn = MODE != kForward;
-    constexpr uint32_t kA = BM * 128, kB = BN * 128;           // one plane of a chunk
+    constexpr int BL = kPair ? BN / 2 : BN;                    // rows of B that this CTA loads
+    constexpr uint32_t kA = BM * 128, kB = BL * 128;           // one plane of a chunk
     constexpr uint32_t kStage = PLANES * (kA + kB);
     constexpr uint32_t kAcc = PLANES == 3 ? 2 * BN : BN;       // TMEM columns of one accumulator (pair)
     constexpr uint32_t kCols = 2 * kAcc;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], fixed[kMaxStages], t_full[2], t_empty[2], drain;
+    __shared__ uint64_t full[kMaxStages], empty[kMaxStages], t_full[2], t_empty[2], drain;
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s;
+    __shared__ uint32_t issued[2];            // pair: chunks that each CTA's loads have begun
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = kPair ? cluster_rank() : 0u;
     float *staging = reinterpret_cast<float *>(smem + (size_t)a.stages * kStage);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
-            mbar_init(&fixed[s], 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&t_full[b], 1);
-            mbar_init(&t_empty[b], 4);
+            mbar_init(&t_empty[b], kPair ? 8 : 4);
         }
         mbar_init(&drain, 1);
         abort_s = 0;
@@ -220,20 +328,18 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
         prefetch_tmap(&bmap);
     }
     lay_out(a.offsets, a.experts, a.rows, off, pre, [&](int32_t n) {
-        if (MODE != kGradW) return (n + BM - 1) / BM;
+        if (MODE != kGradW) return (n + Walk<MODE, BN, kPair>::kRows - 1) / Walk<MODE, BN, kPair>::kRows;
         // an expert without rows still has its gradient (zeros) to write when nothing joins parts
         return n == 0 ? (a.split ? 0 : 1) : (n + a.chunk_rows - 1) / a.chunk_rows;
     });
-    if (warp == 0) {
-        tmem_alloc(&tmem_s, kCols);
-        tmem_relinquish();
-    }
+    if (warp == 0) tmem_take<kPair>(&tmem_s, kCols);
     tc_fence_before();
     __syncthreads();
+    if (kPair) cluster_sync();                // the other CTA's barriers are set up
     tc_fence_after();
     const uint32_t tmem = tmem_s;
     volatile int *abort_flag = &abort_s;
-    Walk<MODE, BN> walk(a, c, off, pre);
+    Walk<MODE, BN, kPair> walk(a, c, off, pre);
     Tile q;
 
     if (warp == 0) {
@@ -243,44 +349,58 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
             bool ok = true;
             while (ok && !*abort_flag && walk.next(q)) {
                 const int blocks = MODE == kGradW ? (int)((q.r1 - q.r0 + BK - 1) / BK) : 0;
+                const int m0 = q.m0 + (int)rank * BM, n0 = q.n0 + (int)rank * BL;
+                const int64_t r0 = q.r0 + (MODE == kGradW ? 0 : rank * BM);
                 for (int kc = 0; kc < q.nk; kc++, u++) {
                     const int s = (int)(u % a.stages);
-                    if (u >= (uint32_t)a.stages && !mbar_wait(&empty[s], ((u / a.stages) - 1) & 1u, abort_flag, a.wait_ns)) {
+                    if (u >= (uint32_t)a.stages && !wait<kPair>(&empty[s], ((u / a.stages) - 1) & 1u, abort_flag, a.wait_ns)) {
                         ok = false;
                         break;
                     }
                     uint8_t *st = smem + (size_t)s * kStage;
-                    mbar_arrive_expect_tx(&full[s], kStage);
+                    // a pair's chunk is complete in the first CTA's barrier, when both halves have landed
+                    const uint32_t bar = kPair ? smem_at(&full[s], 0) : smem_u32(&full[s]);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (kPair ? 2 : 1) * kStage);
 #pragma unroll
                     for (int pl = 0; pl < PLANES; pl++) {
                         uint8_t *sa = st + pl * kA, *sb = st + PLANES * kA + pl * kB;
                         if (MODE == kGradW) {
-                            const int p = c.first[q.p] + kc / blocks, r = (int)q.r0 + (kc % blocks) * BK;
+                            const int p = c.first[q.p] + kc / blocks, rb = kc % blocks;
+                            const bool tail = q.r0 + (int64_t)(rb + 1) * BK > q.r1;
+                            const int r = tail ? q.e * BK : (int)q.r0 + rb * BK;
+                            const CUtensorMap *am = tail ? &atail : &amap, *bm = tail ? &btail : &bmap;
 #pragma unroll
-                            for (int i = 0; i < BM / 64; i++) tma_load_4d(sa + i * kBox, &amap, q.m0 + i * 64, p, r, pl, &full[s]);
+                            for (int i = 0; i < BM / 64; i++) tma_load_4d<kPair>(sa + i * kBox, am, m0 + i * 64, p, r, pl, bar);
 #pragma unroll
-                            for (int i = 0; i < BN / 64; i++) tma_load_4d(sb + i * kBox, &bmap, q.n0 + i * 64, p, r, pl, &full[s]);
+                            for (int i = 0; i < BL / 64; i++) tma_load_4d<kPair>(sb + i * kBox, bm, n0 + i * 64, p, r, pl, bar);
                         } else {
-                            tma_load_4d(sa, &amap, kc * BK, q.p, (int)q.r0, pl, &full[s]);
+                            tma_load_4d<kPair>(sa, &amap, kc * BK, q.p, (int)r0, pl, bar);
                             const int wi = q.e * c.reps + c.rep[q.p];
                             if (kBmn) {
 #pragma unroll
-                                for (int i = 0; i < BN / 64; i++)
-                                    tma_load_4d(sb + i * kBox, &bmap, q.n0 + i * 64, kc * BK, wi, pl, &full[s]);
+                                for (int i = 0; i < BL / 64; i++)
+                                    tma_load_4d<kPair>(sb + i * kBox, &bmap, n0 + i * 64, kc * BK, wi, pl, bar);
                             } else {
-                                tma_load_4d(sb, &bmap, kc * BK, q.n0, wi, pl, &full[s]);
+                                tma_load_4d<kPair>(sb, &bmap, kc * BK, n0, wi, pl, bar);
                             }
                         }
                     }
                 }
             }
-            // every copy issued has landed before the CTA leaves
-            for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
-                mbar_wait_drain(&full[v % a.stages], (v / a.stages) & 1u);
+            if (!kPair) {
+                // every copy issued has landed before the CTA leaves
+                for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
+                    mbar_wait_drain(&full[v % a.stages], (v / a.stages) & 1u);
+            } else {
+                // every signal that the first CTA sends to this one's ring has come, or the pair gives up
+                for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
+                    if (!wait<kPair>(&empty[v % a.stages], (v / a.stages) & 1u, abort_flag, a.wait_ns)) break;
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(smem_at(&issued[rank], 0)), "r"(u) : "memory");
+            }
         }
     } else if (warp == 1) {
-        // ---------------- products ----------------
-        if (lane == 0) {
+        // ---------------- products (pair: the first CTA issues them for both) ----------------
+        if (lane == 0 && rank == 0) {
             uint32_t u = 0, used = 0;
             bool ok = true;
             while (ok && !*abort_flag && walk.next(q)) {
@@ -290,7 +410,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                     const bool first = PLANES == 3 ? kc % kSegment == 0 : kc == 0;
                     if (first) {
                         buf = (int)(used & 1);
-                        if (used >= 2 && !mbar_wait(&t_empty[buf], ((used >> 1) - 1) & 1u, abort_flag, a.wait_ns)) {
+                        if (used >= 2 && !wait<kPair>(&t_empty[buf], ((used >> 1) - 1) & 1u, abort_flag, a.wait_ns)) {
                             ok = false;
                             break;
                         }
@@ -299,8 +419,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                         d = tmem + (uint32_t)buf * kAcc;
                     }
                     const int s = (int)(u % a.stages);
-                    uint64_t *ready = MODE == kGradW ? &fixed[s] : &full[s];
-                    if (!mbar_wait(ready, (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
+                    if (!wait<kPair>(&full[s], (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
                         ok = false;
                         break;
                     }
@@ -315,21 +434,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
 #pragma unroll
                         for (int i = 0; i < kPairs; i++) {
                             const uint32_t aa = ao + pa[i] * kA, bb = bo + pb[i] * kB;
-                            umma_f16(i == 0 ? d : d + BN, kAmn ? smem_desc_mn(aa) : smem_desc_sw128(aa),
-                                     kBmn ? smem_desc_mn(bb) : smem_desc_sw128(bb), a.idesc,
-                                     first && ks == 0 && i <= 1 ? 0u : 1u);
+                            mma<kPair>(i == 0 ? d : d + BN, kAmn ? smem_desc_mn(aa) : smem_desc_sw128(aa),
+                                       kBmn ? smem_desc_mn(bb) : smem_desc_sw128(bb), a.idesc,
+                                       first && ks == 0 && i <= 1 ? 0u : 1u);
                         }
                     }
-                    umma_commit(&empty[s]);
-                    if (kc == q.nk - 1 || (PLANES == 3 && kc % kSegment == kSegment - 1)) umma_commit(&t_full[buf]);
+                    commit<kPair>(&empty[s]);
+                    if (kc == q.nk - 1 || (PLANES == 3 && kc % kSegment == kSegment - 1)) commit<kPair>(&t_full[buf]);
                 }
             }
-            umma_commit(&drain);
+            if (kPair)                        // this CTA's barrier only
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                             ::"r"(smem_u32(&drain)) : "memory");
+            else
+                umma_commit(&drain);
             mbar_wait_drain(&drain, 0);
         }
     } else if (warp < 6) {
         // ---------------- epilogue ----------------
         const int quad = warp & 3;
+        auto tmem_free = [](uint64_t *bar) {
+            if (kPair) mbar_arrive_at(smem_at(bar, 0));
+            else mbar_arrive(bar);
+        };
         float *st = staging + quad * 32 * kStageLd;
         const int es = a.out_dtype == FEQ_DTYPE_F32 ? 4 : 2;
         const int ld = MODE == kGradW ? a.K : a.J, cols = ld;
@@ -355,7 +482,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 for (int i = 0; i < (PLANES == 3 ? BN : 1); i++) acc[i] = 0.0f;
                 for (int kc = 0; kc < q.nk; kc += kSegment, used++) {
                     const int buf = (int)(used & 1);
-                    if (!mbar_wait(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) {
+                    if (!wait<kPair>(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) {
                         ok = false;
                         break;
                     }
@@ -372,10 +499,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&t_empty[buf]);
+                    if (lane == 0) tmem_free(&t_empty[buf]);
                 }
             } else if (q.nk > 0) {
-                ok = mbar_wait(&t_full[used & 1], (used >> 1) & 1u, abort_flag, a.wait_ns);
+                ok = wait<kPair>(&t_full[used & 1], (used >> 1) & 1u, abort_flag, a.wait_ns);
                 tc_fence_after();
             }
             if (!ok) break;
@@ -383,14 +510,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
             // row i of this warp's 32 rows: valid below `live`, at out + i * pitch
             int live;
             int64_t at, pitch;
+            const int below = (int)rank * BM + quad * 32;          // rows of the tile before this warp's
             if (MODE == kGradW) {
-                live = min(32, max(0, a.J - q.m0 - quad * 32));
+                live = min(32, max(0, a.J - q.m0 - below));
                 const int64_t unit = a.split ? q.part : (int64_t)q.e * c.reps + q.p;
-                at = (unit * a.J + q.m0 + quad * 32) * ld;
+                at = (unit * a.J + q.m0 + below) * ld;
                 pitch = ld;
             } else {
-                live = (int)max64(0, min64(32, q.r1 - q.r0 - quad * 32));
-                at = ((q.r0 + quad * 32) * c.dim + q.p) * (int64_t)ld;
+                live = (int)max64(0, min64(32, q.r1 - q.r0 - below));
+                at = ((q.r0 + below) * c.dim + q.p) * (int64_t)ld;
                 pitch = (int64_t)c.dim * ld;
             }
 #pragma unroll (PLANES == 3 ? BN / 32 : 1)
@@ -480,43 +608,63 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
             if (PLANES == 1 && q.nk > 0) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&t_empty[used & 1]);
+                if (lane == 0) tmem_free(&t_empty[used & 1]);
                 used++;
             }
         }
-    } else if (MODE == kGradW) {
-        // ---------------- rows of a chunk that belong to the next expert ----------------
-        uint32_t u = 0;
-        bool ok = true;
-        while (ok && !*abort_flag && walk.next(q)) {
-            const int blocks = (int)((q.r1 - q.r0 + BK - 1) / BK), live = (int)((q.r1 - q.r0) % BK);
-            for (int kc = 0; kc < q.nk; kc++, u++) {
-                const int s = (int)(u % a.stages);
-                if (!mbar_wait(&full[s], (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
-                    ok = false;
-                    break;
-                }
-                if (live != 0 && kc % blocks == blocks - 1) {
-                    // a k row is 128 bytes of every box; the swizzle moves data within a row only
-                    uint8_t *st = smem + (size_t)s * kStage;
-                    const int per = (BK - live) * 8;                 // 16-byte pieces of a box
-                    for (int i = lane; i < per * (int)(kStage / kBox); i += 32) {
-                        const int box = i / per, j = i - box * per;
-                        *reinterpret_cast<uint4 *>(st + box * kBox + live * 128 + j * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&fixed[s]);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (kPair) {
+        cluster_sync();
+        // Copies in flight when the pair gave up: a chunk begun by one CTA only is completed here for the
+        // other one, then every chunk's copies are waited for.
+        if (rank == 0 && threadIdx.x == 0) {
+            const uint32_t u0 = issued[0], u1 = issued[1], last = max(u0, u1);
+            for (uint32_t v = last > (uint32_t)a.stages ? last - a.stages : 0; v < last; v++) {
+                uint64_t *bar = &full[v % a.stages];
+                if (v >= u1)
+                    asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                                 "r"(kStage) : "memory");
+                if (v >= u0) mbar_arrive_expect_tx(bar, kStage);
+                mbar_wait_drain(bar, (v / a.stages) & 1u);
             }
         }
+        cluster_sync();                       // nothing of a CTA is read or signalled by the other any more
     }
-    __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        tmem_dealloc(tmem, kCols);
+        tmem_give<kPair>(tmem, kCols);
     }
     if (threadIdx.x == 0 && abort_s) set_status(a.status, 2);
+}
+
+// The rows of each expert that do not fill a chunk of 64, padded with rows of zeros: (planes, experts * 64,
+// dim, np) from (planes, rows, dim, n) 16-bit values, np a multiple of 8.  One block a row of the result.
+__global__ void __launch_bounds__(256)
+tails_kernel(const uint16_t *__restrict__ src, int64_t row, int64_t comp, int64_t plane, int planes, int dim, int n, int np,
+             const int32_t *__restrict__ offsets, int experts, int64_t rows, uint16_t *__restrict__ dst) {
+    const int e = blockIdx.x / BK, i = blockIdx.x % BK;
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
+    lay_out(offsets, experts, rows, off, pre, [](int32_t) { return 0; });
+    const int live = (off[e + 1] - off[e]) % BK;
+    if (live == 0) return;                    // this expert has no such chunk: nothing reads it
+    const int64_t r = off[e + 1] - live + i;
+    const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uint64_t)(row | comp | plane) * 2) & 15) == 0;
+    const int units = np / 8;
+    for (int u = threadIdx.x; u < planes * dim * units; u += 256) {
+        const int pl = u / (dim * units), d = u / units % dim, k0 = u % units * 8;
+        const uint16_t *s = src + pl * plane + r * row + d * comp + k0;
+        Pack<uint16_t, 8> o;
+        if (i < live && wide && k0 + 8 <= n) {
+            o = *reinterpret_cast<const Pack<uint16_t, 8> *>(s);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; q++) o.v[q] = i < live && k0 + q < n ? s[q] : (uint16_t)0;
+        }
+        *reinterpret_cast<Pack<uint16_t, 8> *>(
+            dst + (((int64_t)pl * experts * BK + blockIdx.x) * dim + d) * np + k0) = o;
+    }
 }
 
 // An expert's partial sums added up in their order: parts of chunk_rows rows, `per` vectors of `size`
@@ -668,6 +816,15 @@ static EncodeFn encode_fn() {
 
 static int pad8(int n) { return (n + 7) & ~7; }
 
+// Makes the current device's context the thread's: tensor maps are encoded by the driver, which a thread
+// without any runtime call behind it (autograd's) has not met yet.
+static int bind_context() {
+    int dev = 0;
+    FEQ_CUDA_TRY(cudaGetDevice(&dev));
+    FEQ_CUDA_TRY(cudaSetDevice(dev));
+    return FEQ_OK;
+}
+
 // A (planes, rows, dim, n) 16-bit tensor as the kernels read it.
 struct Operand {
     const void *base;
@@ -691,7 +848,10 @@ static int make_map(CUtensorMap *m, const Operand &o, int box_mid, int box_rows)
                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        record_error_text("cuTensorMapEncodeTiled refused an operand");
+        char text[256];
+        snprintf(text, sizeof(text), "cuTensorMapEncodeTiled returned %d for (%d, %d, %lld, %d), strides %lld, %lld, %lld at %p",
+                 (int)r, o.n, o.dim, (long long)o.rows, o.planes, (long long)comp, (long long)row, (long long)plane, o.base);
+        record_error_text(text);
         return FEQ_ERR_CUDA;
     }
     return FEQ_OK;
@@ -744,50 +904,105 @@ static int operand(Operand *o, const void *p, int dtype, int64_t rows, int dim, 
     return FEQ_OK;
 }
 
-template <int MODE, int PLANES, int BN>
-static int launch(const CUtensorMap &am, const CUtensorMap &bm, Params a, const Comps &c, int64_t tiles, cudaStream_t s) {
-    constexpr uint32_t stage = PLANES * (BM + BN) * 128;
-    a.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemLimit - 1024 - kStaging) / stage);
-    const uint32_t smem = 1024 + a.stages * stage + kStaging;
-    auto kern = gemm_kernel<MODE, PLANES, BN>;
-    FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    const unsigned grid = (unsigned)max64(1, min64(tiles, sm_count()));
-    kern<<<grid, kThreads, smem, s>>>(am, bm, a, c);
+static size_t tail_bytes(int planes, int experts, int dim, int n) { return (size_t)planes * experts * BK * dim * pad8(n) * 2; }
+
+// The padded last rows of an operand's experts.
+static int tails_of(Operand *t, const Operand &o, const FeqExpertLinearArgs &q, WsCarver *ws, cudaStream_t s) {
+    const int np = pad8(o.n);
+    *t = o;
+    t->rows = (int64_t)q.num_experts * BK;
+    t->comp = np;
+    t->row = (int64_t)o.dim * np;
+    t->plane = t->rows * t->row;
+    t->base = ws->take(tail_bytes(o.planes, q.num_experts, o.dim, o.n));
+    if (ws->used > ws->cap) return FEQ_ERR_WORKSPACE;
+    tails_kernel<<<(unsigned)t->rows, 256, 0, s>>>(static_cast<const uint16_t *>(o.base), o.row, o.comp, o.plane, o.planes,
+                                                   o.dim, o.n, np, q.offsets, q.num_experts, q.rows,
+                                                   static_cast<uint16_t *>(const_cast<void *>(t->base)));
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
 
-// Width of a tile: the widest whose tiles still fill the SMs (a wider tile reads its operands fewer
-// times); float32 keeps three planes of both operands in shared memory, which leaves room for 128.
-static int tile_width(int planes, int64_t row_units, int n) {
-    const int widest = planes == 1 ? 256 : 128;
-    int bn = widest;
-    while (bn > 64 && (n <= bn / 2 || row_units * ((n + bn - 1) / bn) < sm_count())) bn >>= 1;
-    return bn;
+template <int MODE, int PLANES, int BN, bool kPair>
+static int launch(const CUtensorMap *m, Params a, const Comps &c, int64_t tiles, cudaStream_t s) {
+    constexpr uint32_t stage = PLANES * (BM + (kPair ? BN / 2 : BN)) * 128;
+    a.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemLimit - 1024 - kStaging) / stage);
+    const uint32_t smem = 1024 + a.stages * stage + kStaging;
+    auto kern = gemm_kernel<MODE, PLANES, BN, kPair>;
+    FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (!kPair) {
+        const unsigned grid = (unsigned)max64(1, min64(tiles, sm_count()));
+        kern<<<grid, kThreads, smem, s>>>(m[0], m[1], m[2], m[3], a, c);
+        FEQ_LAUNCH_CHECK();
+        return FEQ_OK;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (unsigned)max64(1, min64(tiles, sm_count() / 2)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = 2;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    FEQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, m[0], m[1], m[2], m[3], a, c));
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
 }
 
+// What a product's tiles are: `bn` columns, on one CTA (128 rows) or on a pair (256 rows).
+struct Tiling {
+    int bn;
+    bool pair;
+};
+
+// tails: (gW) the padded last rows of A and B, as maps describe them.
 template <int MODE>
-static int run(const Operand &A, const Operand &B, Params a, const Comps &c, int bn, int64_t tiles, cudaStream_t s) {
-    CUtensorMap am, bm;
-    int rc = MODE == kGradW ? make_map(&am, A, 1, BK) : make_map(&am, A, 1, BM);
-    if (rc != FEQ_OK) return rc;
-    // weights (matrices, c_out, c_in): the middle dimension is c_out
-    rc = MODE == kGradW ? make_map(&bm, B, 1, BK) : make_map(&bm, B, MODE == kForward ? bn : BK, 1);
+static int run(const Operand &A, const Operand &B, const Operand *tails, Params a, const Comps &c, Tiling t, int64_t tiles,
+               cudaStream_t s) {
+    CUtensorMap m[4];
+    int rc;
+    if (MODE == kGradW) {
+        rc = make_map(&m[0], A, 1, BK);
+        if (rc == FEQ_OK) rc = make_map(&m[1], B, 1, BK);
+        if (rc == FEQ_OK) rc = make_map(&m[2], tails[0], 1, BK);
+        if (rc == FEQ_OK) rc = make_map(&m[3], tails[1], 1, BK);
+    } else {
+        rc = make_map(&m[0], A, 1, BM);
+        // weights (matrices, c_out, c_in): the middle dimension is c_out
+        if (rc == FEQ_OK) rc = make_map(&m[1], B, MODE == kForward ? (t.pair ? t.bn / 2 : t.bn) : BK, 1);
+        m[2] = m[0];                          // not used
+        m[3] = m[1];
+    }
     if (rc != FEQ_OK) return rc;
     if (A.planes == 3)
-        return bn == 128 ? launch<MODE, 3, 128>(am, bm, a, c, tiles, s) : launch<MODE, 3, 64>(am, bm, a, c, tiles, s);
-    switch (bn) {
-        case 256: return launch<MODE, 1, 256>(am, bm, a, c, tiles, s);
-        case 128: return launch<MODE, 1, 128>(am, bm, a, c, tiles, s);
-        default: return launch<MODE, 1, 64>(am, bm, a, c, tiles, s);
+        return t.bn == 128 ? launch<MODE, 3, 128, false>(m, a, c, tiles, s) : launch<MODE, 3, 64, false>(m, a, c, tiles, s);
+    if (t.pair) return launch<MODE, 1, 256, true>(m, a, c, tiles, s);
+    switch (t.bn) {
+        case 256: return launch<MODE, 1, 256, false>(m, a, c, tiles, s);
+        case 128: return launch<MODE, 1, 128, false>(m, a, c, tiles, s);
+        default: return launch<MODE, 1, 64, false>(m, a, c, tiles, s);
     }
 }
 
+// Tiles of a row product: the widest whose tiles still fill the SMs (a wider tile reads its operands
+// fewer times); float32 keeps three planes of both operands in shared memory, which leaves room for
+// 128.  Pairs where 256-row tiles of the experts' average rows fill the SMs twice.
+static Tiling row_tiling(int planes, int64_t rows, int experts, int dim, int n) {
+    Tiling t = {planes == 1 ? 256 : 128, false};
+    const int64_t units = (rows + BM - 1) / BM * dim;
+    while (t.bn > 64 && (n <= t.bn / 2 || units * ((n + t.bn - 1) / t.bn) < sm_count())) t.bn >>= 1;
+    t.pair = t.bn == 256 && rows / experts >= 2 * BM && rows / (2 * BM) * dim * ((n + 255) / 256) >= sm_count();
+    return t;
+}
+
 // kind::f16: D float32, A and B of the same 16-bit type, bits 15 / 16 for MN-major operands.
-static uint32_t instr(int dtype, int bn, bool a_mn, bool b_mn) {
+static uint32_t instr(int dtype, Tiling t, bool a_mn, bool b_mn) {
     const uint32_t f = dtype == FEQ_DTYPE_F16 ? 0u : 1u;
     return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+           ((uint32_t)(t.bn >> 3) << 17) | ((uint32_t)((t.pair ? 2 * BM : BM) >> 4) << 24);
 }
 
 int build_comps(const int32_t *lvals, int32_t n, Comps *c) {
@@ -813,20 +1028,30 @@ int check(const FeqExpertLinearArgs &q, Comps *c) {
     return build_comps(q.lvals, q.n_lvals, c);
 }
 
+int64_t grad_w_tiles(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
+    const int high = t.pair ? 2 * BM : BM;
+    return (int64_t)q.num_experts * c.reps * ((q.c_out + high - 1) / high) * ((q.c_in + t.bn - 1) / t.bn);
+}
+
+// Tiles of gW: pairs where they fill the SMs twice without being split.
+Tiling grad_w_tiling(const FeqExpertLinearArgs &q, const Comps &c) {
+    Tiling t = {q.c_in <= 64 ? 64 : q.dtype == FEQ_DTYPE_F32 || q.c_in <= 128 ? 128 : 256, false};
+    if (t.bn == 256 && q.c_out > BM) t.pair = grad_w_tiles(q, c, {256, true}) >= 148;
+    return t;
+}
+
 // Rows of one part of gW's contraction (0: an expert's rows are one part): the whole expert where its
 // tiles fill the SMs anyway, else enough parts for about two tiles a SM, of 256 rows at least; never more
 // than kLongestPart terms, so that the tensor cores' cut-off stays below 1e-4 of a 16-bit sum.
-int part_rows(const FeqExpertLinearArgs &q, const Comps &c, int bn) {
-    const int64_t base = (int64_t)q.num_experts * c.reps * ((q.c_out + BM - 1) / BM) * ((q.c_in + bn - 1) / bn);
-    const int64_t parts = (2 * 148 + base - 1) / base;
+int part_rows(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
+    const int64_t base = grad_w_tiles(q, c, t);
+    const int64_t parts = t.pair ? 1 : (2 * 148 + base - 1) / base;
     int most = 1;
     for (int i = 0; i < c.reps; i++) most = std::max(most, c.first[i + 1] - c.first[i]);
     const int64_t longest = kLongestPart / most / 64 * 64;
     if (parts <= 1) return q.dtype != FEQ_DTYPE_F32 && q.rows > longest ? (int)longest : 0;
     return (int)min64(longest, max64(256, (q.rows / q.num_experts / parts + 63) / 64 * 64));
 }
-
-int grad_w_width(const FeqExpertLinearArgs &q) { return q.dtype == FEQ_DTYPE_F32 || q.c_in <= 128 ? (q.c_in <= 64 ? 64 : 128) : 256; }
 
 }  // namespace elin
 }  // namespace feq
@@ -850,7 +1075,10 @@ static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool 
     if (!backward || q.grad_x) pack(q.weight, matrices, q.c_out, q.c_in, (int64_t)q.c_out * q.c_in, q.c_in);
     if (!backward || q.grad_weight) pack(q.x, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride);
     if (backward && q.grad_weight) {
-        const int part = part_rows(q, c, grad_w_width(q));
+        const int planes = q.dtype == FEQ_DTYPE_F32 ? 3 : 1;
+        ws.take(tail_bytes(planes, q.num_experts, c.dim, q.c_out));
+        ws.take(tail_bytes(planes, q.num_experts, c.dim, q.c_in));
+        const int part = part_rows(q, c, grad_w_tiling(q, c));
         if (part > 0) ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
     }
     if (backward && q.grad_bias && c.scalars)
@@ -906,10 +1134,11 @@ static int row_product(const FeqExpertLinearArgs &q, const Comps &c, const Opera
     a.K = MODE == kForward ? q.c_in : q.c_out;
     a.out = out;
     a.bias = MODE == kForward ? q.bias : nullptr;
-    const int64_t units = ((q.rows + BM - 1) / BM + min64(q.num_experts, q.rows)) * c.dim;
-    const int bn = tile_width(A.planes, (q.rows + BM - 1) / BM * c.dim, a.J);
-    a.idesc = instr(q.dtype, bn, false, MODE == kGradX);
-    return run<MODE>(A, W, a, c, bn, units * ((a.J + bn - 1) / bn), s);
+    const Tiling t = row_tiling(A.planes, q.rows, q.num_experts, c.dim, a.J);
+    const int64_t high = t.pair ? 2 * BM : BM;
+    const int64_t units = ((q.rows + high - 1) / high + min64(q.num_experts, q.rows)) * c.dim;
+    a.idesc = instr(q.dtype, t, false, MODE == kGradX);
+    return run<MODE>(A, W, nullptr, a, c, t, units * ((a.J + t.bn - 1) / t.bn), s);
 }
 
 }  // namespace elin
@@ -926,6 +1155,7 @@ extern "C" int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *work
     if (!q.x || !q.weight || !q.offsets || !q.out) return FEQ_ERR_INVALID_ARGUMENT;
     if (!elin::workspace_ok(workspace, workspace_bytes, elin::workspace_need(q, c, false))) return FEQ_ERR_WORKSPACE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if ((rc = elin::bind_context()) != FEQ_OK) return rc;
     ProfScope prof("expert_linear", s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
     elin::Operand x, w;
@@ -953,6 +1183,7 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
     }
     if (!q.offsets || !q.grad_out || (q.grad_x && !q.weight) || (q.grad_weight && !q.x)) return FEQ_ERR_INVALID_ARGUMENT;
     if (!elin::workspace_ok(workspace, workspace_bytes, elin::workspace_need(q, c, true))) return FEQ_ERR_WORKSPACE;
+    if ((rc = elin::bind_context()) != FEQ_OK) return rc;
     ProfScope prof("expert_linear_bwd", s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
     elin::Operand g, x, w;
@@ -969,7 +1200,8 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
     if (q.grad_weight) {
         rc = elin::operand(&x, q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride, &ws, s);
         if (rc != FEQ_OK) return rc;
-        const int bn = elin::grad_w_width(q), part = elin::part_rows(q, c, bn);
+        const elin::Tiling t = elin::grad_w_tiling(q, c);
+        const int part = elin::part_rows(q, c, t);
         elin::Params a = elin::params(q);
         a.J = q.c_out;
         a.K = q.c_in;
@@ -982,9 +1214,12 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
             if (ws.used > ws.cap) return FEQ_ERR_WORKSPACE;
             a.out_dtype = FEQ_DTYPE_F32;
         }
-        a.idesc = elin::instr(q.dtype, bn, true, true);
-        const int64_t tiles = parts * c.reps * ((q.c_out + elin::BM - 1) / elin::BM) * ((q.c_in + bn - 1) / bn);
-        rc = elin::run<elin::kGradW>(g, x, a, c, bn, tiles, s);
+        a.idesc = elin::instr(q.dtype, t, true, true);
+        const int64_t tiles = parts * (elin::grad_w_tiles(q, c, t) / q.num_experts);
+        elin::Operand tails[2];
+        rc = elin::tails_of(&tails[0], g, q, &ws, s);
+        if (rc == FEQ_OK) rc = elin::tails_of(&tails[1], x, q, &ws, s);
+        if (rc == FEQ_OK) rc = elin::run<elin::kGradW>(g, x, tails, a, c, t, tiles, s);
         if (rc != FEQ_OK) return rc;
         if (a.split) {
             rc = elin::join(static_cast<const float *>(a.out), q, c, part, c.reps, (int64_t)q.c_in * q.c_out,
