@@ -50,8 +50,12 @@ constexpr int kMaxStages = 8;
 constexpr int kSegment = 4;                         // chunks a float32 accumulator runs over
 constexpr int kLongestPart = 65536;                 // terms of one 16-bit sum over rows
 constexpr int kStageLd = 36;                        // floats per row of the epilogue's staging block
-constexpr uint32_t kStaging = 4 * 32 * kStageLd * 4;
+constexpr uint32_t kStaging = 4 * (32 * kStageLd * 4 + 256 * 4);   // a block and a tile's bias for each warp
 constexpr uint32_t kSmemLimit = 227 * 1024 - 6 * 1024;   // dynamic part; barriers and prefixes are static
+__host__ __device__ constexpr uint32_t stages_of(uint32_t stage) {
+    const uint32_t n = (kSmemLimit - 1024 - kStaging) / stage;
+    return n < (uint32_t)kMaxStages ? n : (uint32_t)kMaxStages;
+}
 
 enum Mode { kForward = 0, kGradX = 1, kGradW = 2 };
 
@@ -72,7 +76,6 @@ struct Params {
     void *out;               // gW: the gradient, or (chunk_rows > 0 and split) float32 partial sums
     const void *bias;
     uint32_t idesc;
-    int stages;
     int chunk_rows;          // gW: rows of one contraction part (a multiple of 64)
     int split;               // gW: parts go to partial sums, joined by join_kernel
     int32_t *status;
@@ -299,6 +302,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
     constexpr int BL = kPair ? BN / 2 : BN;                    // rows of B that this CTA loads
     constexpr uint32_t kA = BM * 128, kB = BL * 128;           // one plane of a chunk
     constexpr uint32_t kStage = PLANES * (kA + kB);
+    constexpr uint32_t kStages = stages_of(kStage);
     constexpr uint32_t kAcc = PLANES == 3 ? 2 * BN : BN;       // TMEM columns of one accumulator (pair)
     constexpr uint32_t kCols = 2 * kAcc;
     extern __shared__ uint8_t smem_raw[];
@@ -310,10 +314,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = kPair ? cluster_rank() : 0u;
-    float *staging = reinterpret_cast<float *>(smem + (size_t)a.stages * kStage);
+    float *staging = reinterpret_cast<float *>(smem + kStages * kStage);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; s++) {
+        for (int s = 0; s < (int)kStages; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -345,102 +349,122 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
     if (warp == 0) {
         // ---------------- loads ----------------
         if (lane == 0) {
-            uint32_t u = 0;
+            uint32_t u = 0, s = 0, lap = 0;           // chunks begun; their slot and how often it was used before
             bool ok = true;
+            // a pair's chunk is complete in the first CTA's barrier, when both halves have landed
+            const uint32_t full0 = kPair ? smem_at(full, 0) : smem_u32(full);
             while (ok && !*abort_flag && walk.next(q)) {
-                const int blocks = MODE == kGradW ? (int)((q.r1 - q.r0 + BK - 1) / BK) : 0;
                 const int m0 = q.m0 + (int)rank * BM, n0 = q.n0 + (int)rank * BL;
-                const int64_t r0 = q.r0 + (MODE == kGradW ? 0 : rank * BM);
-                for (int kc = 0; kc < q.nk; kc++, u++) {
-                    const int s = (int)(u % a.stages);
-                    if (u >= (uint32_t)a.stages && !wait<kPair>(&empty[s], ((u / a.stages) - 1) & 1u, abort_flag, a.wait_ns)) {
+                int r = (int)q.r0 + (MODE == kGradW ? 0 : (int)rank * BM), x = 0;
+                int p = MODE == kGradW ? c.first[q.p] : q.p;
+                const int wi = MODE == kGradW ? 0 : q.e * c.reps + c.rep[q.p];
+                for (int kc = 0; kc < q.nk; kc++) {
+                    if (lap > 0 && !wait<kPair>(&empty[s], (lap - 1) & 1u, abort_flag, a.wait_ns)) {
                         ok = false;
                         break;
                     }
-                    uint8_t *st = smem + (size_t)s * kStage;
-                    // a pair's chunk is complete in the first CTA's barrier, when both halves have landed
-                    const uint32_t bar = kPair ? smem_at(&full[s], 0) : smem_u32(&full[s]);
+                    uint8_t *st = smem + s * kStage;
+                    const uint32_t bar = full0 + s * 8;
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], (kPair ? 2 : 1) * kStage);
+                    const bool tail = MODE == kGradW && r + BK > (int)q.r1;
+                    const CUtensorMap *am = tail ? &atail : &amap, *bm = tail ? &btail : &bmap;
+                    const int row = tail ? q.e * BK : r;
 #pragma unroll
                     for (int pl = 0; pl < PLANES; pl++) {
                         uint8_t *sa = st + pl * kA, *sb = st + PLANES * kA + pl * kB;
                         if (MODE == kGradW) {
-                            const int p = c.first[q.p] + kc / blocks, rb = kc % blocks;
-                            const bool tail = q.r0 + (int64_t)(rb + 1) * BK > q.r1;
-                            const int r = tail ? q.e * BK : (int)q.r0 + rb * BK;
-                            const CUtensorMap *am = tail ? &atail : &amap, *bm = tail ? &btail : &bmap;
 #pragma unroll
-                            for (int i = 0; i < BM / 64; i++) tma_load_4d<kPair>(sa + i * kBox, am, m0 + i * 64, p, r, pl, bar);
+                            for (int i = 0; i < BM / 64; i++) tma_load_4d<kPair>(sa + i * kBox, am, m0 + i * 64, p, row, pl, bar);
 #pragma unroll
-                            for (int i = 0; i < BL / 64; i++) tma_load_4d<kPair>(sb + i * kBox, bm, n0 + i * 64, p, r, pl, bar);
+                            for (int i = 0; i < BL / 64; i++) tma_load_4d<kPair>(sb + i * kBox, bm, n0 + i * 64, p, row, pl, bar);
                         } else {
-                            tma_load_4d<kPair>(sa, &amap, kc * BK, q.p, (int)r0, pl, bar);
-                            const int wi = q.e * c.reps + c.rep[q.p];
+                            tma_load_4d<kPair>(sa, &amap, x, p, r, pl, bar);
                             if (kBmn) {
 #pragma unroll
                                 for (int i = 0; i < BL / 64; i++)
-                                    tma_load_4d<kPair>(sb + i * kBox, &bmap, n0 + i * 64, kc * BK, wi, pl, bar);
+                                    tma_load_4d<kPair>(sb + i * kBox, &bmap, n0 + i * 64, x, wi, pl, bar);
                             } else {
-                                tma_load_4d<kPair>(sb, &bmap, kc * BK, n0, wi, pl, bar);
+                                tma_load_4d<kPair>(sb, &bmap, x, n0, wi, pl, bar);
                             }
                         }
+                    }
+                    if (MODE == kGradW) {             // the rows of a component, then the next component
+                        r += BK;
+                        if (r >= (int)q.r1) {
+                            r = (int)q.r0;
+                            p++;
+                        }
+                    } else {
+                        x += BK;
+                    }
+                    u++;
+                    if (++s == kStages) {
+                        s = 0;
+                        lap++;
                     }
                 }
             }
             if (!kPair) {
                 // every copy issued has landed before the CTA leaves
-                for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
-                    mbar_wait_drain(&full[v % a.stages], (v / a.stages) & 1u);
+                for (uint32_t v = u > kStages ? u - kStages : 0; v < u; v++)
+                    mbar_wait_drain(&full[v % kStages], (v / kStages) & 1u);
             } else {
                 // every signal that the first CTA sends to this one's ring has come, or the pair gives up
-                for (uint32_t v = u > (uint32_t)a.stages ? u - a.stages : 0; v < u; v++)
-                    if (!wait<kPair>(&empty[v % a.stages], (v / a.stages) & 1u, abort_flag, a.wait_ns)) break;
+                for (uint32_t v = u > kStages ? u - kStages : 0; v < u; v++)
+                    if (!wait<kPair>(&empty[v % kStages], (v / kStages) & 1u, abort_flag, a.wait_ns)) break;
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(smem_at(&issued[rank], 0)), "r"(u) : "memory");
             }
         }
     } else if (warp == 1) {
         // ---------------- products (pair: the first CTA issues them for both) ----------------
+        // One thread issues everything, so what it computes between two products is what they wait for: the
+        // descriptors are a base and constants, slots and phases are counted, not divided.
         if (lane == 0 && rank == 0) {
-            uint32_t u = 0, used = 0;
+            uint32_t used = 0, s = 0, phase = 0;
             bool ok = true;
+            const uint64_t a0 = kAmn ? smem_desc_mn(smem_u32(smem)) : smem_desc_sw128(smem_u32(smem));
+            const uint64_t b0 = kBmn ? smem_desc_mn(smem_u32(smem) + PLANES * kA) : smem_desc_sw128(smem_u32(smem) + PLANES * kA);
+            constexpr uint32_t kStepA = (kAmn ? 2048 : 32) >> 4, kStepB = (kBmn ? 2048 : 32) >> 4;   // 16 of K
             while (ok && !*abort_flag && walk.next(q)) {
-                uint32_t d = 0;
-                int buf = 0;
-                for (int kc = 0; kc < q.nk; kc++, u++) {
-                    const bool first = PLANES == 3 ? kc % kSegment == 0 : kc == 0;
-                    if (first) {
-                        buf = (int)(used & 1);
+                uint32_t d = 0, begun = 0, buf = 0;
+                int seg = 0;
+                for (int kc = 0; kc < q.nk; kc++) {
+                    if (seg == 0) {
+                        buf = used & 1;
                         if (used >= 2 && !wait<kPair>(&t_empty[buf], ((used >> 1) - 1) & 1u, abort_flag, a.wait_ns)) {
                             ok = false;
                             break;
                         }
                         used++;
                         tc_fence_after();
-                        d = tmem + (uint32_t)buf * kAcc;
+                        d = tmem + buf * kAcc;
+                        begun = 0;
                     }
-                    const int s = (int)(u % a.stages);
-                    if (!wait<kPair>(&full[s], (u / a.stages) & 1u, abort_flag, a.wait_ns)) {
+                    if (!wait<kPair>(&full[s], phase, abort_flag, a.wait_ns)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + (size_t)s * kStage), sb = sa + PLANES * kA;
+                    const uint64_t ad = a0 + s * (kStage >> 4), bd = b0 + s * (kStage >> 4);
 #pragma unroll
                     for (int ks = 0; ks < BK / 16; ks++) {
-                        const uint32_t ao = sa + (kAmn ? ks * 2048 : ks * 32), bo = sb + (kBmn ? ks * 2048 : ks * 32);
                         // planes: hi hi, then (three planes) the five smaller products
                         constexpr int kPairs = PLANES == 1 ? 1 : 6;
-                        constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+                        constexpr uint32_t pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
 #pragma unroll
-                        for (int i = 0; i < kPairs; i++) {
-                            const uint32_t aa = ao + pa[i] * kA, bb = bo + pb[i] * kB;
-                            mma<kPair>(i == 0 ? d : d + BN, kAmn ? smem_desc_mn(aa) : smem_desc_sw128(aa),
-                                       kBmn ? smem_desc_mn(bb) : smem_desc_sw128(bb), a.idesc,
-                                       first && ks == 0 && i <= 1 ? 0u : 1u);
-                        }
+                        for (int i = 0; i < kPairs; i++)
+                            mma<kPair>(i == 0 ? d : d + BN, ad + (ks * kStepA + pa[i] * (kA >> 4)),
+                                       bd + (ks * kStepB + pb[i] * (kB >> 4)), a.idesc, ks > 0 || i > 1 ? 1u : begun);
                     }
+                    begun = 1;
                     commit<kPair>(&empty[s]);
-                    if (kc == q.nk - 1 || (PLANES == 3 && kc % kSegment == kSegment - 1)) commit<kPair>(&t_full[buf]);
+                    if (++s == kStages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                    if (PLANES == 3 && ++seg == kSegment) seg = 0;
+                    if (PLANES == 1) seg = 1;
+                    if (kc == q.nk - 1 || (PLANES == 3 && seg == 0)) commit<kPair>(&t_full[buf]);
                 }
             }
             if (kPair)                        // this CTA's barrier only
@@ -457,7 +481,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
             if (kPair) mbar_arrive_at(smem_at(bar, 0));
             else mbar_arrive(bar);
         };
-        float *st = staging + quad * 32 * kStageLd;
+        float *st = staging + quad * 32 * kStageLd, *bias_s = staging + 4 * 32 * kStageLd + quad * 256;
         const int es = a.out_dtype == FEQ_DTYPE_F32 ? 4 : 2;
         const int ld = MODE == kGradW ? a.K : a.J, cols = ld;
         const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)ld * es) & 15) == 0;
@@ -475,6 +499,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
         }
         uint32_t used = 0;
         while (!*abort_flag && walk.next(q)) {
+            const int sc = MODE == kForward && a.bias ? c.scalar_of[c.rep[q.p]] : -1;
+            if (MODE == kForward) {           // the tile's bias, while its products run
+                __syncwarp();
+                for (int i = lane; i < BN; i += 32) {
+                    const int64_t at = ((int64_t)q.e * c.scalars + sc) * a.J + q.n0 + i;
+                    float b = 0.0f;
+                    if (sc >= 0 && q.n0 + i < a.J)
+                        b = a.bias_dtype == FEQ_DTYPE_F32 ? static_cast<const float *>(a.bias)[at]
+                            : a.bias_dtype == FEQ_DTYPE_BF16 ? to_f32(static_cast<const __nv_bfloat16 *>(a.bias)[at])
+                                                             : to_f32(static_cast<const __half *>(a.bias)[at]);
+                    bias_s[i] = b;
+                }
+                __syncwarp();
+            }
             float acc[PLANES == 3 ? BN : 1];
             bool ok = true;
             if (PLANES == 3) {
@@ -506,7 +544,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 tc_fence_after();
             }
             if (!ok) break;
-            const int sc = MODE == kForward && a.bias ? c.scalar_of[c.rep[q.p]] : -1;
             // row i of this warp's 32 rows: valid below `live`, at out + i * pitch
             int live;
             int64_t at, pitch;
@@ -520,6 +557,67 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 live = (int)max64(0, min64(32, q.r1 - q.r0 - below));
                 at = ((q.r0 + below) * c.dim + q.p) * (int64_t)ld;
                 pitch = (int64_t)c.dim * ld;
+            }
+            if (PLANES == 1 && es == 2 && vec && q.nk > 0) {
+                // 16-bit rows, 64 columns at a time: rounded in the registers, then a block of 32 rows x 128 B
+                // through shared memory to stores of whole rows
+                const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (used & 1) * kAcc;
+                uint8_t *sb = reinterpret_cast<uint8_t *>(st);
+                uint16_t *o = static_cast<uint16_t *>(a.out) + at + (lane >> 3) * pitch + q.n0 + (lane & 7) * 8;
+                const bool bf = a.out_dtype == FEQ_DTYPE_BF16;
+                const int n = min(BN, cols - q.n0);
+#pragma unroll 1
+                for (int c0 = 0; c0 < n; c0 += 64) {
+                    uint32_t v[2][32];
+                    tmem_ld32(t + c0, v[0]);
+                    tmem_ld32(t + c0 + 32, v[1]);
+                    tmem_wait_ld();
+                    if (c0 + 64 >= n) {       // the accumulator is read: the next tile may have it
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tmem_free(&t_empty[used & 1]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            float f[8];
+#pragma unroll
+                            for (int k = 0; k < 8; k++) f[k] = __uint_as_float(v[h][i + k]);
+                            if (MODE == kForward) {
+                                const float4 b0 = *reinterpret_cast<const float4 *>(bias_s + c0 + h * 32 + i);
+                                const float4 b1 = *reinterpret_cast<const float4 *>(bias_s + c0 + h * 32 + i + 4);
+                                f[0] += b0.x, f[1] += b0.y, f[2] += b0.z, f[3] += b0.w;
+                                f[4] += b1.x, f[5] += b1.y, f[6] += b1.z, f[7] += b1.w;
+                            }
+                            uint32_t r[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                if (bf) {
+                                    const __nv_bfloat162 w = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+                                    r[k] = *reinterpret_cast<const uint32_t *>(&w);
+                                } else {
+                                    const __half2 w = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+                                    r[k] = *reinterpret_cast<const uint32_t *>(&w);
+                                }
+                            }
+                            *reinterpret_cast<uint4 *>(sb + lane * (kStageLd * 4) + (h * 32 + i) * 2) =
+                                make_uint4(r[0], r[1], r[2], r[3]);
+                        }
+                    __syncwarp();
+                    if (c0 + (lane & 7) * 8 < n) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const int row = i * 4 + (lane >> 3);
+                            if (row < live)
+                                *reinterpret_cast<uint4 *>(o + i * 4 * pitch + c0) =
+                                    *reinterpret_cast<const uint4 *>(sb + row * (kStageLd * 4) + (lane & 7) * 16);
+                        }
+                    }
+                }
+                used++;
+                continue;
             }
 #pragma unroll (PLANES == 3 ? BN / 32 : 1)
             for (int c0 = 0; c0 < BN; c0 += 32) {
@@ -540,16 +638,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 for (int i = 0; i < 32; i += 4)
                     *reinterpret_cast<uint4 *>(st + lane * kStageLd + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                 __syncwarp();
-                auto bias_at = [&](int col) -> float {
-                    if (sc < 0 || col >= cols) return 0.0f;
-                    const int64_t i = ((int64_t)q.e * c.scalars + sc) * a.J + col;
-                    return a.bias_dtype == FEQ_DTYPE_F32 ? static_cast<const float *>(a.bias)[i]
-                           : a.bias_dtype == FEQ_DTYPE_BF16 ? to_f32(static_cast<const __nv_bfloat16 *>(a.bias)[i])
-                                                            : to_f32(static_cast<const __half *>(a.bias)[i]);
-                };
+                auto bias_at = [&](int i) -> float { return MODE == kForward ? bias_s[c0 + i] : 0.0f; };
                 if (vec && es == 4) {
                     const int cc = (lane & 7) * 4, col = q.n0 + c0 + cc;
-                    const float b0 = bias_at(col), b1 = bias_at(col + 1), b2 = bias_at(col + 2), b3 = bias_at(col + 3);
+                    const float b0 = bias_at(cc), b1 = bias_at(cc + 1), b2 = bias_at(cc + 2), b3 = bias_at(cc + 3);
                     float *o = static_cast<float *>(a.out) + at + col;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
@@ -561,36 +653,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                         f.w += b3;
                         if (row < live && col < cols) *reinterpret_cast<float4 *>(o + row * pitch) = f;
                     }
-                } else if (vec) {
-                    const int cc = (lane & 3) * 8, col = q.n0 + c0 + cc;
-                    float b[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) b[i] = bias_at(col + i);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int row = i * 8 + (lane >> 2);
-                        const float4 f = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc);
-                        const float4 g = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc + 4);
-                        const float w[8] = {f.x + b[0], f.y + b[1], f.z + b[2], f.w + b[3],
-                                            g.x + b[4], g.y + b[5], g.z + b[6], g.w + b[7]};
-                        if (row < live && col < cols) {
-                            if (a.out_dtype == FEQ_DTYPE_BF16) {
-                                Pack<__nv_bfloat16, 8> o;
-#pragma unroll
-                                for (int k = 0; k < 8; k++) o.v[k] = from_f32<__nv_bfloat16>(w[k]);
-                                *reinterpret_cast<Pack<__nv_bfloat16, 8> *>(static_cast<__nv_bfloat16 *>(a.out) + at +
-                                                                           row * pitch + col) = o;
-                            } else {
-                                Pack<__half, 8> o;
-#pragma unroll
-                                for (int k = 0; k < 8; k++) o.v[k] = from_f32<__half>(w[k]);
-                                *reinterpret_cast<Pack<__half, 8> *>(static_cast<__half *>(a.out) + at + row * pitch + col) = o;
-                            }
-                        }
-                    }
                 } else {
                     const int col = q.n0 + c0 + lane;
-                    const float b = bias_at(col);
+                    const float b = bias_at(lane);
                     if (col < cols) {
                         for (int row = 0; row < live; row++) {
                             const float w = st[row * kStageLd + lane] + b;
@@ -621,13 +686,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
         // other one, then every chunk's copies are waited for.
         if (rank == 0 && threadIdx.x == 0) {
             const uint32_t u0 = issued[0], u1 = issued[1], last = max(u0, u1);
-            for (uint32_t v = last > (uint32_t)a.stages ? last - a.stages : 0; v < last; v++) {
-                uint64_t *bar = &full[v % a.stages];
+            for (uint32_t v = last > kStages ? last - kStages : 0; v < last; v++) {
+                uint64_t *bar = &full[v % kStages];
                 if (v >= u1)
                     asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
                                  "r"(kStage) : "memory");
                 if (v >= u0) mbar_arrive_expect_tx(bar, kStage);
-                mbar_wait_drain(bar, (v / a.stages) & 1u);
+                mbar_wait_drain(bar, (v / kStages) & 1u);
             }
         }
         cluster_sync();                       // nothing of a CTA is read or signalled by the other any more
@@ -926,8 +991,7 @@ static int tails_of(Operand *t, const Operand &o, const FeqExpertLinearArgs &q, 
 template <int MODE, int PLANES, int BN, bool kPair>
 static int launch(const CUtensorMap *m, Params a, const Comps &c, int64_t tiles, cudaStream_t s) {
     constexpr uint32_t stage = PLANES * (BM + (kPair ? BN / 2 : BN)) * 128;
-    a.stages = (int)std::min<uint32_t>(kMaxStages, (kSmemLimit - 1024 - kStaging) / stage);
-    const uint32_t smem = 1024 + a.stages * stage + kStaging;
+    constexpr uint32_t smem = 1024 + stages_of(stage) * stage + kStaging;
     auto kern = gemm_kernel<MODE, PLANES, BN, kPair>;
     FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (!kPair) {
