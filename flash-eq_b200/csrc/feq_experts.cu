@@ -340,8 +340,9 @@ struct Rows {
     const void *a, *b;                        // read: token rows (a), sorted rows (b)
     void *out;
     int64_t tokens, a_stride, b_stride;
-    int top_k, experts;
-    int64_t width;                            // elements of a row
+    int top_k, experts, tpr;                  // tpr: lanes of a token
+    int64_t width, units;                     // elements and vectors of a row
+    uint64_t inv_units;                       // ceil(2^64 / units), 0 where units is 1
     const int32_t *slots, *offsets;
     const float *w;
     float *gw;
@@ -356,92 +357,147 @@ __device__ __forceinline__ int place_of(const Rows &a, int64_t pair, int kept) {
     return slot < kept ? slot : kNoExpert;
 }
 
+// dispatch sees the token rows as one line of units of V elements, so that rows of any width keep all
+// lanes busy; a thread has kUnits of them, a block apart, in flight.
+constexpr int kRowThreads = 256, kUnits = 4;
+
+// Unit i: token i / units, found with the multiplier ceil(2^64 / units); exact while i * units < 2^64.
+__device__ __forceinline__ int64_t token_of(const Rows &a, int64_t i) {
+    return a.inv_units ? (int64_t)__umul64hi((uint64_t)i, a.inv_units) : i;
+}
+
 // The token's row goes to its top_k places (x[n] -> sorted); pairs without an expert get zeros.
-// A unit is `V` elements of one token: units of a row lie side by side.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) dispatch_kernel(const Rows a) {
-    const int64_t units = a.width / V, total = a.tokens * units;
+__global__ void __launch_bounds__(kRowThreads) dispatch_kernel(const Rows a) {
+    constexpr int U = kUnits;
     const int kept = a.offsets[a.experts];
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = i / units, c = (i - n * units) * V;
-        const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.a) + n * a.a_stride + c);
-        Pack<T, V> z;
+    Pack<T, V> zero, v[U];
+    int64_t n[U], c[U];
 #pragma unroll
-        for (int q = 0; q < V; q++) z.v[q] = from_f32<T>(0.0f);
-        for (int j = 0; j < a.top_k; j++) {
-            const int64_t slot = a.slots[n * a.top_k + j];
-            const int at = place_of(a, n * a.top_k + j, kept);
-            if (at == kOutside) continue;
-            *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + slot * a.width + c) = at >= 0 ? v : z;
+    for (int q = 0; q < V; q++) zero.v[q] = from_f32<T>(0.0f);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int64_t i = ((int64_t)blockIdx.x * U + u) * kRowThreads + threadIdx.x;
+        n[u] = token_of(a, i);
+        c[u] = (i - n[u] * a.units) * V;
+        v[u] = zero;
+        if (n[u] < a.tokens) v[u] = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.a) + n[u] * a.a_stride + c[u]);
+    }
+    for (int j = 0; j < a.top_k; j++) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (n[u] >= a.tokens) continue;
+            const int place = place_of(a, n[u] * a.top_k + j, kept);
+            if (place == kOutside) continue;
+            *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + (int64_t)a.slots[n[u] * a.top_k + j] * a.width + c[u]) =
+                place >= 0 ? v[u] : zero;
         }
     }
+}
+
+// combine and its backward give a token to `tpr` neighbouring lanes (a power of two up to 32), which
+// share the reads of its slots and weights; K choices are taken together, so that their rows are in flight
+// at once.
+struct Lanes {
+    int64_t n, step;
+    int t, tpr;
+};
+__device__ __forceinline__ Lanes lanes_of(int tpr) {
+    return {(int64_t)blockIdx.x * (kRowThreads / tpr) + threadIdx.x / tpr, (int64_t)gridDim.x * (kRowThreads / tpr),
+            (int)threadIdx.x & (tpr - 1), tpr};
 }
 
 // out[n] = sum_j w[n, j] sorted[slots[n, j]] (w null: 1), summed in float32 in the order of j.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) combine_kernel(const Rows a) {
-    const int64_t units = a.width / V, total = a.tokens * units;
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kRowThreads) combine_kernel(const Rows a) {
     const int kept = a.offsets[a.experts];
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = i / units, c = (i - n * units) * V;
-        float s[V];
+    for (Lanes at = lanes_of(a.tpr); at.n < a.tokens; at.n += at.step) {
+        for (int64_t c = at.t * V; c < a.width; c += at.tpr * V) {
+            float s[V];
 #pragma unroll
-        for (int q = 0; q < V; q++) s[q] = 0.0f;
-        for (int j = 0; j < a.top_k; j++) {
-            const int64_t p = n * a.top_k + j;
-            const int64_t slot = place_of(a, p, kept);
-            if (slot < 0) continue;
-            const Pack<T, V> v =
-                *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.b) + slot * a.b_stride + c);
-            const float w = a.w ? a.w[p] : 1.0f;
+            for (int q = 0; q < V; q++) s[q] = 0.0f;
+            for (int j0 = 0; j0 < a.top_k; j0 += K) {
+                int place[K];
 #pragma unroll
-            for (int q = 0; q < V; q++) s[q] += w * to_f32(v.v[q]);
+                for (int j = 0; j < K; j++)
+                    place[j] = j0 + j < a.top_k ? place_of(a, at.n * a.top_k + j0 + j, kept) : (int)kNoExpert;
+                // the loads do not wait for one another's condition: a pair without an expert reads row 0 and
+                // leaves it
+                Pack<T, V> v[K];
+#pragma unroll
+                for (int j = 0; j < K; j++)
+                    v[j] = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.b) +
+                                                                 max(place[j], 0) * a.b_stride + c);
+#pragma unroll
+                for (int j = 0; j < K; j++) {
+                    if (place[j] < 0) continue;
+                    const float w = a.w ? a.w[at.n * a.top_k + j0 + j] : 1.0f;
+#pragma unroll
+                    for (int q = 0; q < V; q++) s[q] += w * to_f32(v[j].v[q]);
+                }
+            }
+            Pack<T, V> o;
+#pragma unroll
+            for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(s[q]);
+            *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + at.n * a.width + c) = o;
         }
-        Pack<T, V> o;
-#pragma unroll
-        for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(s[q]);
-        *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + n * a.width + c) = o;
     }
 }
 
-// grad_y[slot] = w grad_out[n] and grad_w = <grad_out[n], y[slot]>: one warp per token.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) combine_bwd_kernel(const Rows a) {
-    const int lane = threadIdx.x & 31;
+// grad_y[slot] = w grad_out[n] and grad_w = <grad_out[n], y[slot]>.  K is 2 where a vector is up to 4
+// elements, 1 where it is 8: two rows of those take the registers of half the warps (131072 x 4 rows of 1024
+// bfloat16: 575 against 410 us; 65536 x 4 of 1024 float32: 405 against 439).
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const Rows a) {
     const int kept = a.offsets[a.experts];
-    for (int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); n < a.tokens; n += (int64_t)gridDim.x * 8) {
-        const T *g = static_cast<const T *>(a.a) + n * a.a_stride;
-        for (int j = 0; j < a.top_k; j++) {
-            const int64_t p = n * a.top_k + j;
-            const int64_t slot = a.slots[p];
-            const int at = place_of(a, p, kept);
-            if (at == kOutside) {
-                if (lane == 0) a.gw[p] = 0.0f;
-                continue;
-            }
-            const bool live = at >= 0;
-            const T *y = static_cast<const T *>(a.b) + slot * a.b_stride;
-            T *out = static_cast<T *>(a.out) + slot * a.width;
-            const float w = a.w[p];
-            float dot = 0.0f;
-            for (int64_t c = lane * V; c < a.width; c += 32 * V) {
-                Pack<T, V> o;
+    Lanes at = lanes_of(a.tpr);
+    // every lane of a warp makes the same number of rounds: the sums are warp-wide
+    const int64_t warp_first = at.n - (threadIdx.x & 31) / at.tpr;
+    for (int64_t n0 = warp_first; n0 < a.tokens; n0 += at.step, at.n += at.step) {
+        const bool here = at.n < a.tokens;
+        const T *g = static_cast<const T *>(a.a) + (here ? at.n * a.a_stride : 0);
+        for (int j0 = 0; j0 < a.top_k; j0 += K) {
+            float dot[K], w[K];
+            int place[K];
+            int64_t slot[K];
 #pragma unroll
-                for (int q = 0; q < V; q++) o.v[q] = from_f32<T>(0.0f);
-                if (live) {
-                    const Pack<T, V> u = *reinterpret_cast<const Pack<T, V> *>(g + c);
-                    const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(y + c);
+            for (int j = 0; j < K; j++) {
+                const int64_t p = at.n * a.top_k + j0 + j;
+                const bool is = here && j0 + j < a.top_k;
+                place[j] = is ? place_of(a, p, kept) : (int)kOutside;
+                slot[j] = is ? a.slots[p] : 0;
+                w[j] = is ? a.w[p] : 0.0f;
+                dot[j] = 0.0f;
+            }
+            for (int64_t c = here ? at.t * V : a.width; c < a.width; c += at.tpr * V) {
+                const Pack<T, V> u = *reinterpret_cast<const Pack<T, V> *>(g + c);
+                Pack<T, V> v[K];
+#pragma unroll
+                for (int j = 0; j < K; j++)      // (row 0 where there is none; not used)
+                    v[j] = *reinterpret_cast<const Pack<T, V> *>(static_cast<const T *>(a.b) +
+                                                                 max(place[j], 0) * a.b_stride + c);
+#pragma unroll
+                for (int j = 0; j < K; j++) {
+                    if (place[j] == kOutside) continue;
+                    Pack<T, V> o;
 #pragma unroll
                     for (int q = 0; q < V; q++) {
-                        const float f = to_f32(u.v[q]);
-                        dot += f * to_f32(v.v[q]);
-                        o.v[q] = from_f32<T>(w * f);
+                        float f = 0.0f;
+                        if (place[j] >= 0) {
+                            f = to_f32(u.v[q]);
+                            dot[j] += f * to_f32(v[j].v[q]);
+                            f *= w[j];
+                        }
+                        o.v[q] = from_f32<T>(f);
                     }
+                    *reinterpret_cast<Pack<T, V> *>(static_cast<T *>(a.out) + slot[j] * a.width + c) = o;
                 }
-                *reinterpret_cast<Pack<T, V> *>(out + c) = o;
             }
-            dot = lane_sum(dot, 32);
-            if (lane == 0) a.gw[p] = dot;
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                dot[j] = lane_sum(dot[j], at.tpr);
+                if (at.t == 0 && here && j0 + j < a.top_k) a.gw[at.n * a.top_k + j0 + j] = dot[j];
+            }
         }
     }
 }
@@ -461,7 +517,19 @@ int check(int64_t tokens, int top_k, int experts) {
     return FEQ_OK;
 }
 
-unsigned row_grid(int64_t units) { return (unsigned)max64(1, min64((units + 255) / 256, (int64_t)sm_count() * 16)); }
+// Blocks of kernels on units, `together` of them a thread.
+unsigned unit_grid(Rows *r, int vec, int together) {
+    r->units = r->width / vec;
+    r->inv_units = r->units > 1 ? ~uint64_t(0) / (uint64_t)r->units + 1 : 0;
+    return (unsigned)((r->tokens * r->units + kRowThreads * together - 1) / (kRowThreads * together));
+}
+
+// Lanes of a token for rows of `units` vectors, and the blocks for it.
+unsigned row_grid(Rows *r, int64_t units) {
+    r->tpr = pow2_ceil(min64(units, 32));
+    const int64_t per = kRowThreads / r->tpr;
+    return (unsigned)max64(1, min64((r->tokens + per - 1) / per, (int64_t)1 << 20));
+}
 
 }  // namespace experts
 }  // namespace feq
@@ -555,6 +623,7 @@ static int rows_args(Rows *r, int64_t tokens, int32_t top_k, int32_t num_experts
                      const int32_t *slots, const int32_t *offsets) {
     const int rc = check(tokens, top_k, num_experts);
     if (rc != FEQ_OK) return rc;
+    if (width >= (int64_t)1 << 24) return FEQ_ERR_UNSUPPORTED;
     if (width < 1 || !dtype_ok(dtype) || !offsets || (tokens && !slots)) return FEQ_ERR_INVALID_ARGUMENT;
     r->tokens = tokens;
     r->top_k = top_k;
@@ -584,8 +653,10 @@ extern "C" int feq_expert_dispatch(const void *x, int64_t tokens, int64_t x_stri
     const size_t es = dtype_bytes(dtype);
     const int vec = vector_elems((uint64_t)(uintptr_t)x | (uint64_t)(uintptr_t)sorted | (uint64_t)x_stride * es |
                                      (uint64_t)width * es, es);
-    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::dispatch_kernel<T, V><<<experts::row_grid(tokens * (width / V)),
-                                                                             256, 0, s>>>(r);))
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, {
+        const unsigned grid = experts::unit_grid(&r, V, experts::kUnits);
+        experts::dispatch_kernel<T, V><<<grid, experts::kRowThreads, 0, s>>>(r);
+    }))
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
@@ -608,8 +679,12 @@ extern "C" int feq_expert_combine(const void *sorted, int64_t sorted_stride, int
     const size_t es = dtype_bytes(dtype);
     const int vec = vector_elems((uint64_t)(uintptr_t)sorted | (uint64_t)(uintptr_t)out |
                                      (uint64_t)sorted_stride * es | (uint64_t)width * es, es);
-    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::combine_kernel<T, V><<<experts::row_grid(tokens * (width / V)),
-                                                                            256, 0, s>>>(r);))
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, {
+        const unsigned grid = experts::row_grid(&r, width / V);
+        auto kern = top_k == 1 ? experts::combine_kernel<T, V, 1> : top_k == 2 ? experts::combine_kernel<T, V, 2>
+                                                                             : experts::combine_kernel<T, V, 4>;
+        kern<<<grid, experts::kRowThreads, 0, s>>>(r);
+    }))
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
@@ -638,8 +713,12 @@ extern "C" int feq_expert_combine_bwd(const void *grad_out, int64_t grad_stride,
     const int vec = vector_elems((uint64_t)(uintptr_t)grad_out | (uint64_t)(uintptr_t)sorted |
                                      (uint64_t)(uintptr_t)grad_sorted | (uint64_t)grad_stride * es |
                                      (uint64_t)sorted_stride * es | (uint64_t)width * es, es);
-    const unsigned grid = (unsigned)min64((tokens + 7) / 8, (int64_t)sm_count() * 32);
-    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, experts::combine_bwd_kernel<T, V><<<grid, 256, 0, s>>>(r);))
+    FEQ_TOKEN_TYPE(dtype, FEQ_TOKEN_VEC(T, vec, {
+        const unsigned grid = experts::row_grid(&r, width / V);
+        constexpr int K = V == 8 ? 1 : 2;
+        auto kern = experts::combine_bwd_kernel<T, V, K>;
+        kern<<<grid, experts::kRowThreads, 0, s>>>(r);
+    }))
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
