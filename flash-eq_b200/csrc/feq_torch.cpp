@@ -1,0 +1,548 @@
+// feq_torch.cpp -- the host side of the layer norm and mixture-of-experts operators: argument checks,
+// outputs and workspace from torch's allocator, calls of the C ABI on the current stream, and
+// autograd, as one Python extension module (flash_eq/_lib/_feq_token.so).
+//
+// These operators run for a few microseconds at small sizes.  A forward and backward pass of a layer norm
+// took 126 us of host time through ctypes and torch.autograd.Function in Python; it is native here for
+// that reason.  Python wraps every function once (flash_eq/cuda/token_ops.py, token_autograd.py).
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <sstream>
+
+#include "flasheq_b200.h"
+
+namespace {
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+using MaybeTensor = std::optional<Tensor>;
+
+template <typename... A>
+std::string text(const A &...a) {
+    std::ostringstream s;
+    (s << ... << a);
+    return s.str();
+}
+template <typename... A>
+[[noreturn]] void value_error(const A &...a) { throw py::value_error(text(a...)); }
+template <typename... A>
+[[noreturn]] void type_error(const A &...a) { throw py::type_error(text(a...)); }
+
+std::string lvals_text(const std::vector<int64_t> &v) {
+    std::string s = "[";
+    for (size_t i = 0; i < v.size(); i++) s += (i ? ", " : "") + std::to_string(v[i]);
+    return s + "]";
+}
+
+Tensor given(const MaybeTensor &t) { return t.has_value() ? *t : Tensor(); }
+void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+int dtype_of(const Tensor &t, const char *name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return FEQ_DTYPE_F32;
+        case at::kBFloat16: return FEQ_DTYPE_BF16;
+        case at::kHalf: return FEQ_DTYPE_F16;
+        default: type_error(name, ": expected float32, bfloat16 or float16; got ", t.scalar_type());
+    }
+}
+
+// Every tensor on one CUDA device (a tensor on the CPU, or on another device, is a RuntimeError).
+template <typename... T>
+void one_device(const Tensor &first, const T &...others) {
+    auto check = [&](const Tensor &t) {
+        if (!t.defined()) return;
+        if (!t.is_cuda()) throw std::runtime_error(text("flash-eq ops need CUDA tensors; got a tensor on ", t.device()));
+        if (t.device() != first.device())
+            throw std::runtime_error(text("flash-eq ops need all tensors on one device; got ", first.device(), " and ", t.device()));
+    };
+    check(first);
+    (check(others), ...);
+}
+
+void ok(int rc, const char *what) {
+    if (rc == FEQ_OK) return;
+    const char *more = feq_last_error();
+    throw std::runtime_error(text(what, " failed: ", feq_status_string(rc), more && *more ? text(" (", more, ")") : ""));
+}
+
+feq_stream_t stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+Tensor workspace(size_t bytes, const Tensor &like) {
+    return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+size_t bytes_of(const Tensor &ws) { return ws.defined() ? (size_t)ws.numel() : 0; }
+
+// (rows, width) with a contiguous last dimension.
+Tensor rows_of(const Tensor &t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// What torch's once_differentiable does: a result that raises when it is differentiated again.
+variable_list once(variable_list grads) {
+    if (!c10::GradMode::is_enabled()) return grads;
+    auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked once_differentiable", (int64_t)grads.size());
+    for (auto &g : grads)
+        if (g.defined()) g = g.detach().requires_grad_();
+    return (*error)(std::move(grads));
+}
+
+// Whether the gradient of the optional argument behind `before` tensors is asked for.  An argument that was
+// not given has no edge, so the ones behind it move up.
+bool wants(AutogradContext *ctx, bool is_there, size_t before) { return is_there && ctx->needs_input_grad(before); }
+
+bool tracks(const Tensor &t) { return t.defined() && t.requires_grad(); }
+template <typename... T>
+bool tracking(const T &...t) { return c10::GradMode::is_enabled() && (tracks(t) || ...); }
+
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+Tensor parameter(const Tensor &p, const Tensor &x, int64_t width, const char *name) {
+    if (!p.defined()) return p;
+    if (p.dim() != 1 || p.size(0) != width) value_error(name, " must have shape (", width, ",); got ", p.sizes());
+    if (p.scalar_type() != x.scalar_type() && p.scalar_type() != at::kFloat)
+        type_error(name, " must be ", x.scalar_type(), " or float32; got ", p.scalar_type());
+    return p.contiguous();
+}
+
+// (y, stats); stats (2, rows) = mean and 1 / std, undefined unless asked for.
+std::pair<Tensor, Tensor> norm_fwd(const Tensor &x, const Tensor &weight, const Tensor &bias, double eps, bool keep) {
+    one_device(x, weight, bias);
+    const int dtype = dtype_of(x, "x");
+    const int64_t width = x.dim() ? x.size(-1) : 0;
+    if (width < 1) value_error("x must have a last dimension of at least 1; got ", x.sizes());
+    if (!(eps >= 0.0)) value_error("eps must be >= 0; got ", eps);
+    const Tensor w = parameter(weight, x, width, "weight"), b = parameter(bias, x, width, "bias");
+    if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
+        type_error("weight and bias must have one type; got ", w.scalar_type(), " and ", b.scalar_type());
+    const Tensor rows = rows_of(x.dim() == 2 ? x : x.reshape({-1, width}));
+    const int64_t n = rows.size(0);
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = at::empty(x.sizes(), x.options()), stats;
+    if (keep) stats = at::empty({2, n}, x.options().dtype(at::kFloat));
+    float *mean = keep ? stats.data_ptr<float>() : nullptr;
+    const Tensor &p = w.defined() ? w : b;
+    ok(feq_layer_norm_fwd(rows.data_ptr(), n, rows.stride(0), (int32_t)std::min<int64_t>(width, INT32_MAX), dtype, ptr(w),
+                          ptr(b), p.defined() && p.scalar_type() == at::kFloat, (float)eps, y.data_ptr(), mean,
+                          keep ? mean + n : nullptr, stream_of(x)),
+       "feq_layer_norm_fwd");
+    return {y, stats};
+}
+
+variable_list norm_bwd(const Tensor &grad, const Tensor &x, const Tensor &weight, const Tensor &stats, bool need_x,
+                       bool need_w, bool need_b, at::ScalarType param) {
+    one_device(grad, x, weight);
+    const int64_t width = x.size(-1);
+    const Tensor rows = rows_of(x.dim() == 2 ? x : x.reshape({-1, width}));
+    const Tensor g = rows_of(grad.dim() == 2 ? grad : grad.reshape({-1, width}));
+    const Tensor w = weight.defined() ? weight.contiguous() : weight;
+    const int64_t n = rows.size(0);
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor gx, gw, gb;
+    if (need_x) gx = at::empty(x.sizes(), x.options());
+    if (need_w) gw = at::empty({width}, x.options().dtype(param));
+    if (need_b) gb = at::empty({width}, x.options().dtype(param));
+    const Tensor ws = workspace(need_w || need_b ? feq_layer_norm_bwd_workspace_bytes(n, (int32_t)width) : 0, x);
+    const float *mean = stats.data_ptr<float>();
+    ok(feq_layer_norm_bwd(g.data_ptr(), g.stride(0), rows.data_ptr(), n, rows.stride(0), (int32_t)width, dtype_of(x, "x"),
+                          ptr(w), param == at::kFloat, mean, mean + n, ptr(gx), ptr(gw), ptr(gb), ptr(ws), bytes_of(ws),
+                          stream_of(x)),
+       "feq_layer_norm_bwd");
+    return {gx, gw, gb};
+}
+
+struct LayerNorm : Function<LayerNorm> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias,
+                          double eps) {
+        const Tensor w = given(weight), b = given(bias);
+        auto [y, stats] = norm_fwd(x, w, b, eps, true);
+        ctx->save_for_backward({x, w, stats});
+        const Tensor &p = w.defined() ? w : b;
+        ctx->saved_data["weight"] = w.defined();
+        ctx->saved_data["bias"] = b.defined();
+        ctx->saved_data["param"] = (int64_t)(p.defined() ? p.scalar_type() : x.scalar_type());
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        variable_list r;
+        {
+            at::AutoGradMode off(false);
+            const bool w = ctx->saved_data["weight"].toBool(), b = ctx->saved_data["bias"].toBool();
+            r = norm_bwd(g[0], s[0], s[1], s[2], ctx->needs_input_grad(0), wants(ctx, w, 1), wants(ctx, b, 1 + w),
+                         (at::ScalarType)ctx->saved_data["param"].toInt());
+        }
+        r.emplace_back();
+        return once(std::move(r));
+    }
+};
+
+Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, double eps) {
+    const Tensor w = given(weight), b = given(bias);
+    if (tracking(x, w, b)) return LayerNorm::apply(x, weight, bias, eps);
+    return norm_fwd(x, w, b, eps, false).first;
+}
+
+// ---------------------------------------------------------------------------
+// expert routing
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxExperts = 512, kMaxTopK = 32;
+
+struct Routed {
+    Tensor ids, weights, slots, offsets;
+};
+
+Routed route_fwd(const Tensor &logits, int64_t k, bool normalize) {
+    one_device(logits);
+    const int dtype = dtype_of(logits, "logits");
+    if (logits.dim() != 2 || logits.size(1) < 1) value_error("logits must be (tokens, num_experts); got ", logits.sizes());
+    const int64_t n = logits.size(0), e = logits.size(1);
+    if (k < 1 || k > e) value_error("top_k must be in [1, num_experts = ", e, "]; got ", k);
+    if (e > kMaxExperts || k > kMaxTopK)
+        value_error("at most ", kMaxExperts, " experts and top_k ", kMaxTopK, "; got ", e, " and ", k);
+    const Tensor rows = rows_of(logits);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const auto i32 = logits.options().dtype(at::kInt);
+    Routed r = {at::empty({n, k}, i32), at::empty({n, k}, logits.options().dtype(at::kFloat)), at::empty({n, k}, i32),
+                at::empty({e + 1}, i32)};
+    const Tensor ws = workspace(feq_expert_route_workspace_bytes(n, (int32_t)k, (int32_t)e), logits);
+    ok(feq_expert_route(rows.data_ptr(), n, rows.stride(0), (int32_t)e, (int32_t)k, dtype, normalize,
+                        r.ids.data_ptr<int32_t>(), r.weights.data_ptr<float>(), r.slots.data_ptr<int32_t>(),
+                        r.offsets.data_ptr<int32_t>(), ptr(ws), bytes_of(ws), stream_of(logits)),
+       "feq_expert_route");
+    return r;
+}
+
+struct Route : Function<Route> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &logits, int64_t k, bool normalize) {
+        Routed r = route_fwd(logits, k, normalize);
+        ctx->mark_non_differentiable({r.ids, r.slots, r.offsets});
+        ctx->save_for_backward({logits, r.ids, r.weights});
+        ctx->saved_data["normalize"] = normalize;
+        return {r.ids, r.weights, r.slots, r.offsets};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        Tensor out;
+        if (g[1].defined()) {
+            at::AutoGradMode off(false);
+            const Tensor rows = rows_of(s[0]), gw = g[1].to(at::kFloat).contiguous();
+            const c10::cuda::CUDAGuard guard(rows.device());
+            out = at::empty(s[0].sizes(), s[0].options());
+            ok(feq_expert_route_bwd(rows.data_ptr(), rows.size(0), rows.stride(0), (int32_t)rows.size(1),
+                                    (int32_t)s[1].size(1), dtype_of(rows, "logits"), ctx->saved_data["normalize"].toBool(),
+                                    s[1].data_ptr<int32_t>(), s[2].data_ptr<float>(), gw.data_ptr<float>(), out.data_ptr(),
+                                    stream_of(rows)),
+               "feq_expert_route_bwd");
+        }
+        return once({out, Tensor(), Tensor()});
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> expert_route(const Tensor &logits, int64_t k, bool normalize) {
+    if (tracking(logits)) {
+        auto r = Route::apply(logits, k, normalize);
+        return {r[0], r[1], r[2], r[3]};
+    }
+    Routed r = route_fwd(logits, k, normalize);
+    return {r.ids, r.weights, r.slots, r.offsets};
+}
+
+// ---- rows ----
+struct Plan {
+    int64_t n;
+    int32_t k, e;
+};
+
+Plan plan_of(const Tensor &slots, const Tensor &offsets) {
+    if (slots.scalar_type() != at::kInt || slots.dim() != 2 || !slots.is_contiguous())
+        type_error("slots must be a contiguous int32 (tokens, top_k) tensor");
+    if (offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) < 2 || !offsets.is_contiguous())
+        type_error("offsets must be a contiguous int32 (num_experts + 1,) tensor");
+    return {slots.size(0), (int32_t)slots.size(1), (int32_t)offsets.size(0) - 1};
+}
+
+// (rows, ...) with `want` rows as (rows, width).
+Tensor flat_rows(const Tensor &t, int64_t want, const char *name) {
+    if (t.dim() < 2 || t.size(0) != want) value_error(name, " must be (", want, ", width); got ", t.sizes());
+    const Tensor f = t.dim() == 2 ? t : t.flatten(1);
+    if (f.size(1) < 1) value_error(name, " must be (", want, ", width); got ", t.sizes());
+    return rows_of(f);
+}
+Tensor with_rows(const Tensor &like, int64_t rows) {
+    auto sizes = like.sizes().vec();
+    sizes[0] = rows;
+    return at::empty(sizes, like.options());
+}
+
+Tensor dispatch_fwd(const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+    one_device(x, slots, offsets);
+    const Plan p = plan_of(slots, offsets);
+    const int dtype = dtype_of(x, "x");
+    const Tensor rows = flat_rows(x, p.n, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor out = with_rows(x, p.n * p.k);
+    ok(feq_expert_dispatch(rows.data_ptr(), p.n, rows.stride(0), rows.size(1), dtype, p.k, p.e, slots.data_ptr<int32_t>(),
+                           offsets.data_ptr<int32_t>(), out.data_ptr(), stream_of(x)),
+       "feq_expert_dispatch");
+    return out;
+}
+
+Tensor combine_fwd(const Tensor &y, const Tensor &weights, const Tensor &slots, const Tensor &offsets) {
+    one_device(y, weights, slots, offsets);
+    const Plan p = plan_of(slots, offsets);
+    const int dtype = dtype_of(y, "y");
+    const Tensor rows = flat_rows(y, p.n * p.k, "y");
+    Tensor w = weights;
+    if (w.defined()) {
+        if (w.sizes() != slots.sizes() || w.scalar_type() != at::kFloat)
+            value_error("weights must be a float32 ", slots.sizes(), " tensor; got ", w.scalar_type(), " ", w.sizes());
+        w = w.contiguous();
+    }
+    const c10::cuda::CUDAGuard guard(y.device());
+    Tensor out = with_rows(y, p.n);
+    ok(feq_expert_combine(rows.data_ptr(), rows.stride(0), p.n, rows.size(1), dtype, p.k, p.e, slots.data_ptr<int32_t>(),
+                          offsets.data_ptr<int32_t>(), static_cast<const float *>(ptr(w)), out.data_ptr(), stream_of(y)),
+       "feq_expert_combine");
+    return out;
+}
+
+struct Dispatch : Function<Dispatch> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+        ctx->save_for_backward({slots, offsets});
+        return dispatch_fwd(x, slots, offsets);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        Tensor gx;
+        {
+            at::AutoGradMode off(false);
+            gx = combine_fwd(g[0], Tensor(), s[0], s[1]);
+        }
+        return once({gx, Tensor(), Tensor()});
+    }
+};
+
+Tensor expert_dispatch(const Tensor &x, const Tensor &slots, const Tensor &offsets) {
+    return tracking(x) ? Dispatch::apply(x, slots, offsets) : dispatch_fwd(x, slots, offsets);
+}
+
+struct Combine : Function<Combine> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &y, const Tensor &weights, const Tensor &slots,
+                          const Tensor &offsets) {
+        ctx->save_for_backward({y, weights, slots, offsets});
+        return combine_fwd(y, weights, slots, offsets);
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &y = s[0], &slots = s[2], &offsets = s[3];
+        Tensor gy, gw;
+        {
+            at::AutoGradMode off(false);
+            one_device(g[0], y);
+            const Plan p = plan_of(slots, offsets);
+            const Tensor rows = flat_rows(y, p.n * p.k, "y"), go = flat_rows(g[0], p.n, "grad_out"), w = s[1].contiguous();
+            const c10::cuda::CUDAGuard guard(y.device());
+            gy = at::empty(y.sizes(), y.options());
+            gw = at::empty(slots.sizes(), y.options().dtype(at::kFloat));
+            ok(feq_expert_combine_bwd(go.data_ptr(), go.stride(0), rows.data_ptr(), rows.stride(0), p.n, rows.size(1),
+                                      dtype_of(y, "y"), p.k, p.e, slots.data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
+                                      w.data_ptr<float>(), gy.data_ptr(), gw.data_ptr<float>(), stream_of(y)),
+               "feq_expert_combine_bwd");
+        }
+        return once({gy, gw, Tensor(), Tensor()});
+    }
+};
+
+Tensor expert_combine(const Tensor &y, const MaybeTensor &weights, const Tensor &slots, const Tensor &offsets) {
+    const Tensor w = given(weights);
+    return tracking(y, w) ? Combine::apply(y, w, slots, offsets) : combine_fwd(y, w, slots, offsets);
+}
+
+// ---------------------------------------------------------------------------
+// expert linear
+// ---------------------------------------------------------------------------
+struct Linear {
+    FeqExpertLinearArgs a = {};
+    std::vector<int32_t> lvals;
+    Tensor x, weight, offsets;        // kept until the call has returned
+    int64_t scalars = 0;
+    bool plain = false;
+};
+
+// Components of a row, sum(2 l + 1).
+int64_t dim_of(const std::vector<int64_t> &lvals) {
+    int64_t dim = 0;
+    bool good = !lvals.empty();
+    for (const int64_t v : lvals) {
+        good &= v >= 0 && v < (1 << 20);
+        dim += 2 * v + 1;
+    }
+    if (!good) value_error("lvals must be a non-empty list of degrees >= 0; got ", lvals_text(lvals));
+    return dim;
+}
+
+// Shapes, and the arguments that both directions share.  x (rows, dim, c_in) with weight (E, reps, c_out,
+// c_in), or plain x (rows, c_in) with (E, c_out, c_in).
+void linear_args(Linear &l, const Tensor &x, const Tensor &weight, const Tensor &offsets, const std::vector<int64_t> &lvals) {
+    const int dtype = dtype_of(x, "x");
+    const int64_t dim = dim_of(lvals);
+    for (const int64_t v : lvals) {
+        l.scalars += v == 0;
+        l.lvals.push_back((int32_t)std::min<int64_t>(v, INT32_MAX));
+    }
+    l.plain = x.dim() == 2;
+    if (l.plain && (lvals.size() != 1 || lvals[0] != 0))
+        value_error("plain rows (rows, c_in) need lvals (0,); got ", lvals_text(lvals));
+    if (!l.plain && (x.dim() != 3 || x.size(1) != dim))
+        value_error("x must be (rows, ", dim, ", c_in) for lvals ", lvals_text(lvals), "; got ", x.sizes());
+    const int64_t ci = x.size(-1);
+    const bool fits = weight.dim() == (l.plain ? 3 : 4) && weight.size(-1) == ci && ci >= 1 && weight.size(-2) >= 1 &&
+                      weight.size(0) >= 1 && (l.plain || weight.size(1) == (int64_t)lvals.size());
+    if (!fits)
+        value_error("weight must be (num_experts, ", l.plain ? "" : text(lvals.size(), ", "), "c_out, ", ci, "); got ",
+                    weight.sizes());
+    const int64_t e = weight.size(0), co = weight.size(-2);
+    if (e > kMaxExperts) value_error("at most ", kMaxExperts, " experts; got ", e);
+    if (ci > INT32_MAX || co > INT32_MAX) value_error("channels must be below 2^31; got ", ci, " and ", co);
+    if (weight.scalar_type() != x.scalar_type())
+        type_error("weight must have x's type ", x.scalar_type(), "; got ", weight.scalar_type());
+    if (offsets.dim() != 1 || offsets.size(0) != e + 1 ||
+        (offsets.scalar_type() != at::kInt && offsets.scalar_type() != at::kLong))
+        value_error("offsets must be an int32 or int64 (", e + 1, ",) tensor; got ", offsets.scalar_type(), " ", offsets.sizes());
+    l.x = rows_of(x);
+    l.weight = weight.contiguous();
+    l.offsets = offsets.to(at::kInt).contiguous();
+    l.a.x = l.x.data_ptr();
+    l.a.x_row_stride = l.x.stride(0);
+    l.a.x_comp_stride = l.plain ? 0 : l.x.stride(1);
+    l.a.weight = l.weight.data_ptr();
+    l.a.offsets = l.offsets.data_ptr<int32_t>();
+    l.a.rows = x.size(0);
+    l.a.lvals = l.lvals.data();
+    l.a.n_lvals = (int32_t)lvals.size();
+    l.a.num_experts = (int32_t)e;
+    l.a.c_in = (int32_t)ci;
+    l.a.c_out = (int32_t)co;
+    l.a.dtype = dtype;
+}
+
+std::vector<int64_t> bias_shape(const Linear &l) {
+    return l.plain ? std::vector<int64_t>{l.a.num_experts, l.a.c_out}
+                   : std::vector<int64_t>{l.a.num_experts, l.scalars, l.a.c_out};
+}
+
+using LinearCall = int (*)(const FeqExpertLinearArgs *, void *, size_t, feq_stream_t);
+void linear_call(LinearCall call, const char *what, Linear &l, int backward, const Tensor &status) {
+    if (status.defined()) l.a.status = status.data_ptr<int32_t>();
+    int rc = call(&l.a, nullptr, 0, stream_of(l.x));
+    if (rc == FEQ_ERR_WORKSPACE) {            // an operand has to be packed, or sums joined
+        const Tensor ws = workspace(feq_expert_linear_workspace_bytes(&l.a, backward), l.x);
+        rc = call(&l.a, ptr(ws), bytes_of(ws), stream_of(l.x));
+    }
+    ok(rc, what);
+}
+
+Tensor linear_fwd(const Tensor &x, const Tensor &weight, const Tensor &bias, const Tensor &offsets,
+                  const std::vector<int64_t> &lvals, const Tensor &status) {
+    one_device(x, weight, bias, offsets);
+    Linear l;
+    linear_args(l, x, weight, offsets, lvals);
+    Tensor b = bias;
+    if (b.defined()) {
+        if (l.scalars == 0) value_error("a bias needs an l = 0 component; lvals are ", lvals_text(lvals));
+        if (b.sizes() != at::IntArrayRef(bias_shape(l))) value_error("bias must be ", bias_shape(l), "; got ", b.sizes());
+        if (b.scalar_type() != x.scalar_type()) type_error("bias must have x's type ", x.scalar_type(), "; got ", b.scalar_type());
+        b = b.contiguous();
+        l.a.bias = b.data_ptr();
+    }
+    const c10::cuda::CUDAGuard guard(x.device());
+    auto sizes = x.sizes().vec();
+    sizes.back() = l.a.c_out;
+    Tensor out = at::empty(sizes, x.options());
+    l.a.out = out.data_ptr();
+    linear_call(feq_expert_linear_fwd, "feq_expert_linear_fwd", l, 0, status);
+    return out;
+}
+
+variable_list linear_bwd(const Tensor &grad, const Tensor &x, const Tensor &weight, const Tensor &offsets,
+                         const std::vector<int64_t> &lvals, bool need_x, bool need_w, bool need_b, const Tensor &status) {
+    one_device(grad, x, weight, offsets);
+    Linear l;
+    linear_args(l, x, weight, offsets, lvals);
+    const Tensor g = rows_of(grad);
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor gx, gw, gb;
+    if (need_x) gx = at::empty(x.sizes(), x.options());
+    if (need_w) gw = at::empty(weight.sizes(), x.options());
+    if (need_b) gb = at::empty(bias_shape(l), x.options());
+    l.a.grad_out = g.data_ptr();
+    l.a.grad_row_stride = g.stride(0);
+    l.a.grad_comp_stride = l.plain ? 0 : g.stride(1);
+    l.a.grad_x = ptr(gx);
+    l.a.grad_weight = ptr(gw);
+    l.a.grad_bias = ptr(gb);
+    linear_call(feq_expert_linear_bwd, "feq_expert_linear_bwd", l, 1, status);
+    return {gx, gw, gb};
+}
+
+struct ExpertLinear : Function<ExpertLinear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const MaybeTensor &bias,
+                          const Tensor &offsets, const std::vector<int64_t> &lvals) {
+        ctx->save_for_backward({x, weight, offsets});
+        ctx->saved_data["lvals"] = lvals;
+        ctx->saved_data["bias"] = bias.has_value();
+        return linear_fwd(x, weight, given(bias), offsets, lvals, Tensor());
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        variable_list r;
+        {
+            at::AutoGradMode off(false);
+            r = linear_bwd(g[0], s[0], s[1], s[2], ctx->saved_data["lvals"].toIntVector(), ctx->needs_input_grad(0),
+                           ctx->needs_input_grad(1), wants(ctx, ctx->saved_data["bias"].toBool(), 2), Tensor());
+        }
+        r.resize(5);
+        return once(std::move(r));
+    }
+};
+
+Tensor expert_linear(const Tensor &x, const Tensor &weight, const MaybeTensor &bias, const Tensor &offsets,
+                     const std::vector<int64_t> &lvals) {
+    const Tensor b = given(bias);
+    return tracking(x, weight, b) ? ExpertLinear::apply(x, weight, bias, offsets, lvals)
+                                  : linear_fwd(x, weight, b, offsets, lvals, Tensor());
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    const auto free_gil = py::call_guard<py::gil_scoped_release>();
+    m.def("abi_version", &feq_abi_version);
+    m.def("check_degrees", &dim_of);
+    m.def("layer_norm", &layer_norm, free_gil);
+    m.def("expert_route", &expert_route, free_gil);
+    m.def("expert_dispatch", &expert_dispatch, free_gil);
+    m.def("expert_combine", &expert_combine, free_gil);
+    m.def("expert_linear", &expert_linear, free_gil);
+    // one direction, without autograd, with a status word
+    m.def("expert_linear_fwd",
+          [](const Tensor &x, const Tensor &w, const MaybeTensor &b, const Tensor &o, const std::vector<int64_t> &lv,
+             const MaybeTensor &status) {
+              at::AutoGradMode off(false);
+              return linear_fwd(x, w, given(b), o, lv, given(status));
+          }, free_gil);
+    m.def("expert_linear_bwd",
+          [](const Tensor &g, const Tensor &x, const Tensor &w, const Tensor &o, const std::vector<int64_t> &lv, bool need_x,
+             bool need_w, bool need_b, const MaybeTensor &status) {
+              at::AutoGradMode off(false);
+              const auto r = linear_bwd(g, x, w, o, lv, need_x, need_w, need_b, given(status));
+              auto maybe = [](const Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
+              return std::make_tuple(maybe(r[0]), maybe(r[1]), maybe(r[2]));
+          }, free_gil);
+}

@@ -14,7 +14,6 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "_lib", "libflasheq_b200.so")
 
 FEQ_OK = 0
-FEQ_ERR_WORKSPACE = 3
 FEQ_BASIS_MFIRST = 0
 FEQ_BASIS_ROT_TO_EZ = 1
 FEQ_REDUCE = {"sum": 0, "mean": 1, "max": 2}

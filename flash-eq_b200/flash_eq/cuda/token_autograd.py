@@ -6,50 +6,22 @@ expert.  ``expert_dispatch`` brings token rows into that order, ``expert_linear`
 expert's linear map to its rows (equivariant rows (rows, dim, channels) with one weight per irrep,
 or plain rows), and ``expert_combine`` sums the weighted rows back onto their tokens.  The row
 counts of the experts stay on the device: no call synchronises the host.  All sums have a fixed
-order, so results and gradients are reproducible bit for bit.
+order, so results and gradients are reproducible bit for bit.  Gradients are differentiable once.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import token_ops
-
-
-def _tracks(*tensors) -> bool:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = token_ops.layer_norm_fwd(x, weight, bias, eps, keep_stats=True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.param_dtype = next((p.dtype for p in (weight, bias) if p is not None), None)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        x, weight, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*token_ops.layer_norm_bwd(grad_out, x, weight, stats, need[0], need[1], need[2], ctx.param_dtype),
-                None)
+from .token_ops import native
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension, in float32, rounded once
     to x's type (float32, bfloat16, float16).  weight and bias: x's type or float32, or None."""
-    if _tracks(x, weight, bias):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return token_ops.layer_norm_fwd(x, weight, bias, eps, keep_stats=False)[0]
+    return native(x).layer_norm(x, weight, bias, eps)
 
 
 @dataclass
@@ -80,101 +52,25 @@ class ExpertRoute:
         return self.slots.shape[0]
 
 
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_k, normalize):
-        ids, weights, slots, offsets = token_ops.expert_route(logits, top_k, normalize)
-        ctx.mark_non_differentiable(ids, slots, offsets)
-        ctx.save_for_backward(logits, ids, weights)
-        ctx.normalize = normalize
-        return ids, weights, slots, offsets
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, _ids, grad_weights, _slots, _offsets):
-        logits, ids, weights = ctx.saved_tensors
-        return token_ops.expert_route_bwd(logits, ids, weights, grad_weights, ctx.normalize), None, None
-
-
 def expert_route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> ExpertRoute:
     """The ``top_k`` best experts of every token and the order by expert, from logits (tokens,
     num_experts).  Equal logits: the lower expert first; a logit of -inf is never chosen, so masking
-    a token's whole row leaves it without an expert (weight 0, zero rows).  ``normalize``: weights are
-    the softmax over the chosen logits, else the chosen entries of the softmax over all of them."""
-    if _tracks(logits):
-        return ExpertRoute(*_Route.apply(logits, int(top_k), bool(normalize)))
-    return ExpertRoute(*token_ops.expert_route(logits, top_k, normalize))
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, slots, offsets):
-        ctx.save_for_backward(slots, offsets)
-        return token_ops.expert_dispatch(x, slots, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_sorted):
-        slots, offsets = ctx.saved_tensors
-        return token_ops.expert_combine(grad_sorted, slots, offsets), None, None
-
-
-def _flat(t: torch.Tensor, name: str):
-    if t.dim() < 2:
-        raise ValueError(f"{name} must be (rows, ...); got {tuple(t.shape)}")
-    return t if t.dim() == 2 else t.flatten(1)
+    a token's whole row leaves it without an expert (weight 0, zero rows); NaN counts as the largest
+    logit and makes the token's weights NaN.  ``normalize``: weights are the softmax over the chosen
+    logits, else the chosen entries of the softmax over all of them."""
+    return ExpertRoute(*native(logits).expert_route(logits, top_k, normalize))
 
 
 def expert_dispatch(x: torch.Tensor, route: ExpertRoute) -> torch.Tensor:
     """Token rows x (tokens, ...) -> (tokens * top_k, ...) in the order by expert; zeros where a pair
     has no expert.  The gradient sums the copies of a token."""
-    rows = _flat(x, "x")
-    if _tracks(x):
-        out = _Dispatch.apply(rows, route.slots, route.offsets)
-    else:
-        out = token_ops.expert_dispatch(rows, route.slots, route.offsets)
-    return out if x.dim() == 2 else out.view(out.shape[0], *x.shape[1:])
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, weights, slots, offsets):
-        ctx.save_for_backward(y, weights, slots, offsets)
-        return token_ops.expert_combine(y, slots, offsets, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        y, weights, slots, offsets = ctx.saved_tensors
-        gy, gw = token_ops.expert_combine_bwd(grad_out, y, slots, offsets, weights)
-        return gy, gw, None, None
+    return native(x).expert_dispatch(x, route.slots, route.offsets)
 
 
 def expert_combine(y: torch.Tensor, route: ExpertRoute) -> torch.Tensor:
     """Rows y (tokens * top_k, ...) in the order by expert -> (tokens, ...): the sum over a token's
     choices of weight * row.  Differentiable in y and, through route.weights, in the logits."""
-    rows = _flat(y, "y")
-    if _tracks(y, route.weights):
-        out = _Combine.apply(rows, route.weights, route.slots, route.offsets)
-    else:
-        out = token_ops.expert_combine(rows, route.slots, route.offsets, route.weights)
-    return out if y.dim() == 2 else out.view(out.shape[0], *y.shape[1:])
-
-
-class _ExpertLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, offsets, lvals):
-        ctx.save_for_backward(x, weight, offsets)
-        ctx.lvals = lvals
-        return token_ops.expert_linear_fwd(x, weight, bias, offsets, lvals)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        x, weight, offsets = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*token_ops.expert_linear_bwd(grad_out, x, weight, offsets, ctx.lvals, need[0], need[1], need[2]),
-                None, None)
+    return native(y).expert_combine(y, route.weights, route.slots, route.offsets)
 
 
 def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, offsets: torch.Tensor,
@@ -184,9 +80,6 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | No
     Plain rows: x (rows, c_in), weight (num_experts, c_out, c_in), bias (num_experts, c_out) or None.
     Equivariant rows: x (rows, dim, c_in) with dim = sum(2 l + 1) over ``lvals``, weight (num_experts,
     len(lvals), c_out, c_in), bias (num_experts, number of l = 0 irreps, c_out) on the l = 0
-    components.  float32, bfloat16 or float16, one type for all; sums in float32."""
-    if type(lvals) is not tuple:
-        lvals = tuple(int(v) for v in lvals)
-    if _tracks(x, weight, bias):
-        return _ExpertLinear.apply(x, weight, bias, offsets, lvals)
-    return token_ops.expert_linear_fwd(x, weight, bias, offsets, lvals)
+    components.  float32, bfloat16 or float16, one type for all; sums in float32.  An infinite float32
+    input gives NaN in the sums that hold it."""
+    return native(x).expert_linear(x, weight, bias, offsets, lvals)

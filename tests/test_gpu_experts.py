@@ -394,6 +394,31 @@ def test_repeatable_and_on_another_stream(cuda_device, dtype):
     assert all(torch.equal(p, q) for p, q in zip(first, again))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (1, 2)])
+def test_expert_linear_some_gradients_only(cuda_device, which, dtype):
+    x, w, b, offsets, go = _linear_inputs([30, 0, 77], 2, (0, 1), 40, 48, dtype, cuda_device, seed=11)
+    want = _linear_reference(x, w, b, offsets, (0, 1), go)[1:]
+    leaves = [t.requires_grad_(i in which) for i, t in enumerate((x, w, b))]
+    got = torch.autograd.grad(fe.expert_linear(*leaves, offsets, (0, 1)), [leaves[i] for i in which], go)
+    for g, i in zip(got, which):
+        assert rel_l2(g, want[i]) < TOL[dtype]
+
+
+def test_gradients_are_differentiable_once(cuda_device):
+    x, w, b, offsets, go = _linear_inputs([3, 4], 0, (0,), 8, 16, torch.float32, cuda_device)
+    g = torch.autograd.grad(fe.expert_linear(x.requires_grad_(), w, b, offsets), x, go, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    z = torch.randn(6, 4, device=cuda_device, requires_grad=True)
+    r = fe.expert_route(z, 2)
+    g = torch.autograd.grad(r.weights[:, 0].sum(), z, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    assert torch.autograd.grad(fe.expert_dispatch(torch.randn(6, 3, device=cuda_device, requires_grad=True), r).sum(),
+                               z, allow_unused=True) == (None,)
+
+
 def test_expert_linear_empty(cuda_device):
     x, w, b, offsets, go = _linear_inputs([0, 0], 0, (0,), 16, 24, torch.float32, cuda_device)
     leaves = [t.requires_grad_() for t in (x, w, b)]

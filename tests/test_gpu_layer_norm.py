@@ -139,6 +139,28 @@ def test_constant_rows_width_one_and_extremes(cuda_device):
     assert torch.equal(y[keep], clean[keep]) and y[2].isnan().all() and y[4].isnan().all()
 
 
+@pytest.mark.parametrize("which", [(0,), (1,), (2,), (0, 2), (1, 2)])
+def test_some_gradients_only(cuda_device, which):
+    x, w, b, go = _inputs(33, 40, torch.float32, cuda_device, seed=9)
+    want = _reference(x, w, b, go, 1e-5)[1:]
+    leaves = [t.requires_grad_(i in which) for i, t in enumerate((x, w, b))]
+    y = fe.layer_norm(*leaves)
+    got = torch.autograd.grad(y, [leaves[i] for i in which], go)
+    for g, i in zip(got, which):
+        assert rel_l2(g, want[i]) < 1e-5
+    if 2 in which:                                          # no weight: the bias moves up
+        y = fe.layer_norm(x, None, b)
+        assert rel_l2(torch.autograd.grad(y, b, go)[0], go.double().sum(0)) < 1e-5
+
+
+def test_gradients_are_differentiable_once(cuda_device):
+    x, w, b, go = _inputs(5, 12, torch.float32, cuda_device)
+    x.requires_grad_()
+    g = torch.autograd.grad(fe.layer_norm(x, w, b), x, go, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_empty(cuda_device):
     x = torch.empty(0, 16, device=cuda_device, requires_grad=True)
     w = torch.ones(16, device=cuda_device, requires_grad=True)

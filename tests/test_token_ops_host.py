@@ -58,6 +58,20 @@ def test_no_gpu_fails_loudly():
             call()
 
 
+def test_native_module_reports_errors():
+    """Its C++ exceptions arrive as Python ones."""
+    from flash_eq.cuda import token_ops
+
+    m = token_ops.load()
+    assert m.abi_version() == _lib.FEQ_ABI_VERSION
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        m.expert_route(torch.randn(3, 4), 2, True)
+    with pytest.raises(ValueError, match="degrees"):
+        m.check_degrees([0, -1])
+    with pytest.raises(TypeError):
+        m.check_degrees("x")
+
+
 def test_layer_bookkeeping():
     m = fe.EquivariantExperts(fe.Repr([0, 1, 2], 8), num_experts=3, top_k=2, mlp_ratio=2)
     assert m.weight_up.shape == (3, 3, 16, 8) and m.weight_down.shape == (3, 3, 8, 16)
