@@ -11,7 +11,7 @@
 // The three products are one persistent tcgen05 kernel (gemm_kernel), a CTA per SM, 128 x BN tiles:
 //   warp 0      loads: tensor-map copies of 64-deep operand chunks into a ring (no multicast)
 //   warp 1      one thread issues tcgen05.mma kind::f16 into one of two TMEM accumulators
-//   warps 2..5  epilogue: tcgen05.ld, + bias, through shared memory to row-contiguous stores, while
+//   warps 2..9  epilogue: tcgen05.ld, + bias, through shared memory to row-contiguous stores, while
 //               the next tile's products run
 // Large 16-bit products run on pairs of CTAs (cta_group::2, 256 x 256 tiles): each CTA loads its 128 rows
 // of A and half of B's, which takes a third off the traffic through shared memory (writes plus reads,
@@ -44,16 +44,21 @@ using namespace sm100;
 
 constexpr int kMaxExperts = 512;
 constexpr int BM = 128, BK = 64;
-constexpr int kThreads = 6 * 32;
+constexpr int kEpilogueWarps = 8;                   // two for each 32 rows, each half of the columns
+constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr uint32_t kBox = 64 * 128;                 // bytes of a 64-row, 64-channel box
 constexpr int kMaxStages = 8;
 constexpr int kSegment = 4;                         // chunks a float32 accumulator runs over
 constexpr int kLongestPart = 65536;                 // terms of one 16-bit sum over rows
-constexpr int kStageLd = 36;                        // floats per row of the epilogue's staging block
-constexpr uint32_t kStaging = 4 * (32 * kStageLd * 4 + 256 * 4);   // a block and a tile's bias for each warp
+// Staging of an epilogue warp: 32 rows of kBlock floats (float32 tiles, whose operand ring leaves less
+// room, 16 = 64 B of a row; else 32 = 128 B), padded by 16 bytes, and the bias of its columns.
+__host__ __device__ constexpr int block_floats(int planes) { return planes == 3 ? 16 : 32; }
+__host__ __device__ constexpr uint32_t staging_bytes(int planes, int bn) {
+    return kEpilogueWarps * (32 * (block_floats(planes) + 4) * 4 + bn / 2 * 4);
+}
 constexpr uint32_t kSmemLimit = 227 * 1024 - 6 * 1024;   // dynamic part; barriers and prefixes are static
-__host__ __device__ constexpr uint32_t stages_of(uint32_t stage) {
-    const uint32_t n = (kSmemLimit - 1024 - kStaging) / stage;
+__host__ __device__ constexpr uint32_t stages_of(uint32_t stage, uint32_t staging) {
+    const uint32_t n = (kSmemLimit - 1024 - staging) / stage;
     return n < (uint32_t)kMaxStages ? n : (uint32_t)kMaxStages;
 }
 
@@ -64,6 +69,7 @@ struct Comps {
     int dim, reps, scalars;
     int16_t first[kMaxIrreps + 1];                  // first component of each irrep
     int8_t scalar_of[kMaxIrreps];                   // scalar index of an l = 0 irrep, else -1
+    int8_t by_size[kMaxIrreps];                     // irreps, those with the most components first
     int8_t rep[kMaxDim];
 };
 
@@ -248,37 +254,49 @@ struct Tile {
     int part;                // gW: index of the partial sum
 };
 
+// The tiles of a CTA, the same for all its roles.  Tiles are dealt out in rounds, every other one
+// backwards; in gW, where an irrep's tiles cost as many chunks as it has components, the largest irreps
+// come first, so that the CTAs with the long tiles get the short ones of the next round (2707 rows, 5
+// experts, l = 0, 0, 1, 263 x 751: the last CTA ended at 59 500 cycles, the average at 19 300).
 template <int MODE, int BN, bool kPair>
 struct Walk {
     static constexpr int kRows = kPair ? 2 * BM : BM;      // rows of a tile
     const Params &a;
     const Comps &c;
     const int32_t *off, *pre;
-    int e = 0, tiles_n, tiles_m;
-    int64_t t, total;
+    int e = 0, rep = -1, tiles_n, tiles_m, me, ctas;
+    int64_t round = 0, total;
     __device__ Walk(const Params &a_, const Comps &c_, const int32_t *off_, const int32_t *pre_)
         : a(a_), c(c_), off(off_), pre(pre_) {
         tiles_n = ((MODE == kGradW ? a.K : a.J) + BN - 1) / BN;
         tiles_m = MODE == kGradW ? (a.J + kRows - 1) / kRows : 1;
         total = (int64_t)pre[a.experts] * (MODE == kGradW ? c.reps * tiles_m : c.dim) * tiles_n;
-        t = blockIdx.x / (kPair ? 2 : 1);
+        me = (int)blockIdx.x / (kPair ? 2 : 1);
+        ctas = (int)gridDim.x / (kPair ? 2 : 1);
     }
     __device__ bool next(Tile &q) {
-        if (t >= total) return false;
-        int64_t u = t;
-        t += gridDim.x / (kPair ? 2 : 1);
+        int64_t u = round * ctas + (round & 1 ? ctas - 1 - me : me);
+        if (u >= total) return false;
+        round++;
         const int nt = (int)(u % tiles_n);
         u /= tiles_n;
         q.n0 = nt * BN;
+        int unit;
         if (MODE == kGradW) {
             q.m0 = (int)(u % tiles_m) * kRows;
             u /= tiles_m;
+            const int units = pre[a.experts], k = (int)(u / units);
+            unit = (int)(u - (int64_t)k * units);
+            q.p = c.by_size[k];
+            if (k != rep) {
+                rep = k;
+                e = 0;
+            }
         } else {
             q.m0 = 0;
+            q.p = (int)(u % c.dim);
+            unit = (int)(u / c.dim);
         }
-        const int inner = MODE == kGradW ? c.reps : c.dim;
-        q.p = (int)(u % inner);
-        const int unit = (int)(u / inner);
         while (pre[e + 1] <= unit) e++;
         q.e = e;
         const int span = MODE == kGradW ? a.chunk_rows : kRows;
@@ -302,7 +320,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
     constexpr int BL = kPair ? BN / 2 : BN;                    // rows of B that this CTA loads
     constexpr uint32_t kA = BM * 128, kB = BL * 128;           // one plane of a chunk
     constexpr uint32_t kStage = PLANES * (kA + kB);
-    constexpr uint32_t kStages = stages_of(kStage);
+    constexpr uint32_t kStaging = staging_bytes(PLANES, BN), kStages = stages_of(kStage, kStaging);
     constexpr uint32_t kAcc = PLANES == 3 ? 2 * BN : BN;       // TMEM columns of one accumulator (pair)
     constexpr uint32_t kCols = 2 * kAcc;
     extern __shared__ uint8_t smem_raw[];
@@ -323,7 +341,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&t_full[b], 1);
-            mbar_init(&t_empty[b], kPair ? 8 : 4);
+            mbar_init(&t_empty[b], (kPair ? 2 : 1) * kEpilogueWarps);
         }
         mbar_init(&drain, 1);
         abort_s = 0;
@@ -474,38 +492,38 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 umma_commit(&drain);
             mbar_wait_drain(&drain, 0);
         }
-    } else if (warp < 6) {
+    } else {
         // ---------------- epilogue ----------------
-        const int quad = warp & 3;
+        // quad: the 32 rows of the warp (TMEM lanes); half: its columns
+        constexpr int kHalf = BN / 2, kBlock = block_floats(PLANES), kLd = kBlock + 4;
+        const int ew = warp - 2, quad = warp & 3, half = (ew >> 2) * kHalf;
         auto tmem_free = [](uint64_t *bar) {
             if (kPair) mbar_arrive_at(smem_at(bar, 0));
             else mbar_arrive(bar);
         };
-        float *st = staging + quad * 32 * kStageLd, *bias_s = staging + 4 * 32 * kStageLd + quad * 256;
+        float *st = staging + ew * 32 * kLd, *bias_s = staging + kEpilogueWarps * 32 * kLd + ew * kHalf;
         const int es = a.out_dtype == FEQ_DTYPE_F32 ? 4 : 2;
-        const int ld = MODE == kGradW ? a.K : a.J, cols = ld;
+        const int ld = MODE == kGradW ? a.K : a.J;
         const bool vec = ((reinterpret_cast<uintptr_t>(a.out) | (uint64_t)ld * es) & 15) == 0;
         if (MODE != kGradW) {
             // rows that belong to no expert: one contiguous range of zeros
-            const int64_t lo = (int64_t)off[a.experts] * c.dim * ld * es, hi = a.rows * c.dim * (int64_t)ld * es;
-            uint8_t *o = static_cast<uint8_t *>(a.out);
-            const int64_t step = (int64_t)gridDim.x * 128 * es;
-            for (int64_t i = lo + ((int64_t)blockIdx.x * 128 + threadIdx.x - 64) * es; i < hi; i += step) {
-                if (es == 4)
-                    *reinterpret_cast<float *>(o + i) = 0.0f;
-                else
-                    *reinterpret_cast<uint16_t *>(o + i) = 0;
+            constexpr int kThem = kEpilogueWarps * 32;
+            const int64_t lo = (int64_t)off[a.experts] * c.dim * ld, hi = a.rows * c.dim * (int64_t)ld;
+            for (int64_t i = lo + (int64_t)blockIdx.x * kThem + threadIdx.x - 64; i < hi; i += (int64_t)gridDim.x * kThem) {
+                if (es == 4) static_cast<float *>(a.out)[i] = 0.0f;
+                else static_cast<uint16_t *>(a.out)[i] = 0;
             }
         }
         uint32_t used = 0;
         while (!*abort_flag && walk.next(q)) {
+            const int col0 = q.n0 + half, n = min(kHalf, ld - col0);        // this warp's columns (n <= 0: none)
             const int sc = MODE == kForward && a.bias ? c.scalar_of[c.rep[q.p]] : -1;
-            if (MODE == kForward) {           // the tile's bias, while its products run
+            if (MODE == kForward) {           // their bias, while the products run
                 __syncwarp();
-                for (int i = lane; i < BN; i += 32) {
-                    const int64_t at = ((int64_t)q.e * c.scalars + sc) * a.J + q.n0 + i;
+                for (int i = lane; i < kHalf; i += 32) {
+                    const int64_t at = ((int64_t)q.e * c.scalars + sc) * a.J + col0 + i;
                     float b = 0.0f;
-                    if (sc >= 0 && q.n0 + i < a.J)
+                    if (sc >= 0 && i < n)
                         b = a.bias_dtype == FEQ_DTYPE_F32 ? static_cast<const float *>(a.bias)[at]
                             : a.bias_dtype == FEQ_DTYPE_BF16 ? to_f32(static_cast<const __nv_bfloat16 *>(a.bias)[at])
                                                              : to_f32(static_cast<const __half *>(a.bias)[at]);
@@ -513,38 +531,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 }
                 __syncwarp();
             }
-            float acc[PLANES == 3 ? BN : 1];
-            bool ok = true;
-            if (PLANES == 3) {
-#pragma unroll
-                for (int i = 0; i < (PLANES == 3 ? BN : 1); i++) acc[i] = 0.0f;
-                for (int kc = 0; kc < q.nk; kc += kSegment, used++) {
-                    const int buf = (int)(used & 1);
-                    if (!wait<kPair>(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)buf * kAcc;
-#pragma unroll
-                    for (int c0 = 0; c0 < (PLANES == 3 ? BN : 0); c0 += 32) {
-                        uint32_t u[32], w[32];
-                        tmem_ld32(t + c0, u);
-                        tmem_ld32(t + BN + c0, w);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) acc[c0 + i] += __uint_as_float(u[i]) + __uint_as_float(w[i]);
-                    }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) tmem_free(&t_empty[buf]);
-                }
-            } else if (q.nk > 0) {
-                ok = wait<kPair>(&t_full[used & 1], (used >> 1) & 1u, abort_flag, a.wait_ns);
-                tc_fence_after();
-            }
-            if (!ok) break;
-            // row i of this warp's 32 rows: valid below `live`, at out + i * pitch
+            // row i of this warp's 32 rows: valid below `live`, at out + at + i * pitch
             int live;
             int64_t at, pitch;
             const int below = (int)rank * BM + quad * 32;          // rows of the tile before this warp's
@@ -558,123 +545,184 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
                 at = ((q.r0 + below) * c.dim + q.p) * (int64_t)ld;
                 pitch = (int64_t)c.dim * ld;
             }
-            if (PLANES == 1 && es == 2 && vec && q.nk > 0) {
-                // 16-bit rows, 64 columns at a time: rounded in the registers, then a block of 32 rows x 128 B
-                // through shared memory to stores of whole rows
-                const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (used & 1) * kAcc;
+            at += col0;
+
+            // a block of kBlock float32 columns from column c0 on
+            auto put_f32 = [&](int c0, const float (&v)[kBlock]) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kBlock; i += 4)
+                    *reinterpret_cast<float4 *>(st + lane * kLd + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                __syncwarp();
+                float *o = static_cast<float *>(a.out) + at + c0;
+                if (vec) {
+                    constexpr int kPer = kBlock / 4, kRows = 32 / kPer;    // lanes of a row, rows at a time
+                    const int cc = lane % kPer * 4;
+                    if (c0 + cc < n) {
+                        const float4 b = MODE == kForward ? *reinterpret_cast<const float4 *>(bias_s + c0 + cc)
+                                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int i = 0; i < kPer; i++) {
+                            const int row = i * kRows + lane / kPer;
+                            float4 f = *reinterpret_cast<const float4 *>(st + row * kLd + cc);
+                            f.x += b.x, f.y += b.y, f.z += b.z, f.w += b.w;
+                            if (row < live) *reinterpret_cast<float4 *>(o + row * pitch + cc) = f;
+                        }
+                    }
+                } else {
+                    constexpr int kRows = 32 / kBlock;
+                    const int cc = lane % kBlock;
+                    if (c0 + cc < n) {
+                        const float b = MODE == kForward ? bias_s[c0 + cc] : 0.0f;
+#pragma unroll 8
+                        for (int row = lane / kBlock; row < live; row += kRows) o[row * pitch + cc] = st[row * kLd + cc] + b;
+                    }
+                }
+            };
+            // kWide 16-bit columns: rounded in the registers, staged, stored 16 bytes a lane, or 4 where rows do
+            // not start on 16 bytes
+            constexpr int kWide = kHalf < 64 ? kHalf : 64;
+            auto put_16 = [&](int c0, const uint32_t (&v)[kWide]) {
                 uint8_t *sb = reinterpret_cast<uint8_t *>(st);
-                uint16_t *o = static_cast<uint16_t *>(a.out) + at + (lane >> 3) * pitch + q.n0 + (lane & 7) * 8;
                 const bool bf = a.out_dtype == FEQ_DTYPE_BF16;
-                const int n = min(BN, cols - q.n0);
-#pragma unroll 1
-                for (int c0 = 0; c0 < n; c0 += 64) {
-                    uint32_t v[2][32];
-                    tmem_ld32(t + c0, v[0]);
-                    tmem_ld32(t + c0 + 32, v[1]);
-                    tmem_wait_ld();
-                    if (c0 + 64 >= n) {       // the accumulator is read: the next tile may have it
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) tmem_free(&t_empty[used & 1]);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kWide; i += 8) {
+                    float f[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) f[k] = __uint_as_float(v[i + k]);
+                    if (MODE == kForward) {
+                        const float4 b0 = *reinterpret_cast<const float4 *>(bias_s + c0 + i);
+                        const float4 b1 = *reinterpret_cast<const float4 *>(bias_s + c0 + i + 4);
+                        f[0] += b0.x, f[1] += b0.y, f[2] += b0.z, f[3] += b0.w;
+                        f[4] += b1.x, f[5] += b1.y, f[6] += b1.z, f[7] += b1.w;
                     }
-                    __syncwarp();
+                    uint32_t r[4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            float f[8];
-#pragma unroll
-                            for (int k = 0; k < 8; k++) f[k] = __uint_as_float(v[h][i + k]);
-                            if (MODE == kForward) {
-                                const float4 b0 = *reinterpret_cast<const float4 *>(bias_s + c0 + h * 32 + i);
-                                const float4 b1 = *reinterpret_cast<const float4 *>(bias_s + c0 + h * 32 + i + 4);
-                                f[0] += b0.x, f[1] += b0.y, f[2] += b0.z, f[3] += b0.w;
-                                f[4] += b1.x, f[5] += b1.y, f[6] += b1.z, f[7] += b1.w;
-                            }
-                            uint32_t r[4];
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                if (bf) {
-                                    const __nv_bfloat162 w = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
-                                    r[k] = *reinterpret_cast<const uint32_t *>(&w);
-                                } else {
-                                    const __half2 w = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
-                                    r[k] = *reinterpret_cast<const uint32_t *>(&w);
-                                }
-                            }
-                            *reinterpret_cast<uint4 *>(sb + lane * (kStageLd * 4) + (h * 32 + i) * 2) =
-                                make_uint4(r[0], r[1], r[2], r[3]);
+                    for (int k = 0; k < 4; k++) {
+                        if (bf) {
+                            const __nv_bfloat162 w = __floats2bfloat162_rn(f[2 * k], f[2 * k + 1]);
+                            r[k] = *reinterpret_cast<const uint32_t *>(&w);
+                        } else {
+                            const __half2 w = __floats2half2_rn(f[2 * k], f[2 * k + 1]);
+                            r[k] = *reinterpret_cast<const uint32_t *>(&w);
                         }
-                    __syncwarp();
-                    if (c0 + (lane & 7) * 8 < n) {
+                    }
+                    *reinterpret_cast<uint4 *>(sb + lane * (kLd * 4) + i * 2) = make_uint4(r[0], r[1], r[2], r[3]);
+                }
+                __syncwarp();
+                uint16_t *o = static_cast<uint16_t *>(a.out) + at + c0;
+                const int m = min(kWide, n - c0);
+                if (vec) {
+                    constexpr int kPer = kWide / 8, kRows = 32 / kPer;
+                    const int cc = lane % kPer * 8;
+                    if (cc < m) {
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int row = i * 4 + (lane >> 3);
+                        for (int i = 0; i < kPer; i++) {
+                            const int row = i * kRows + lane / kPer;
                             if (row < live)
-                                *reinterpret_cast<uint4 *>(o + i * 4 * pitch + c0) =
-                                    *reinterpret_cast<const uint4 *>(sb + row * (kStageLd * 4) + (lane & 7) * 16);
+                                *reinterpret_cast<uint4 *>(o + row * pitch + cc) =
+                                    *reinterpret_cast<const uint4 *>(sb + row * (kLd * 4) + cc * 2);
+                        }
+                    }
+                } else {
+                    // pairs on 4-byte boundaries; in a row that starts off one, the first element and the last
+                    // alone
+                    constexpr int kPer = kWide / 2, kRows = 32 / kPer;
+                    const int pair = lane % kPer;
+                    const uint32_t start = (uint32_t)(reinterpret_cast<uintptr_t>(o) >> 1), step = (uint32_t)pitch;
+#pragma unroll 4
+                    for (int row = lane / kPer; row < live; row += kRows) {
+                        const uint32_t *in = reinterpret_cast<const uint32_t *>(sb + row * (kLd * 4)) + pair;
+                        const int odd = (int)(start + row * step) & 1, i = 2 * pair + odd;
+                        const uint32_t lo = in[0], w = __funnelshift_r(lo, in[1], odd * 16);
+                        uint16_t *r = o + row * pitch;
+                        if (i + 1 < m) *reinterpret_cast<uint32_t *>(r + i) = w;
+                        else if (i < m) r[i] = (uint16_t)w;
+                        if (odd && pair == 0) r[0] = (uint16_t)lo;
+                    }
+                }
+            };
+
+            if (PLANES == 3) {
+                float acc[PLANES == 3 ? kHalf : 1];
+                bool ok = true;
+#pragma unroll
+                for (int i = 0; i < (PLANES == 3 ? kHalf : 1); i++) acc[i] = 0.0f;
+                for (int kc = 0; kc < q.nk; kc += kSegment, used++) {
+                    const int buf = (int)(used & 1);
+                    if (!wait<kPair>(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t t = tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)buf * kAcc + half;
+#pragma unroll
+                    for (int c0 = 0; c0 < (PLANES == 3 ? kHalf : 0); c0 += 32) {
+                        uint32_t u[32], w[32];
+                        tmem_ld32(t + c0, u);
+                        tmem_ld32(t + BN + c0, w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) acc[c0 + i] += __uint_as_float(u[i]) + __uint_as_float(w[i]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tmem_free(&t_empty[buf]);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c0 = 0; c0 < (PLANES == 3 ? kHalf : 0); c0 += kBlock) {
+                    float v[kBlock];
+#pragma unroll
+                    for (int i = 0; i < kBlock; i++) v[i] = acc[PLANES == 3 ? c0 + i : 0];
+                    if (c0 < n) put_f32(c0, v);
+                }
+            } else {
+                const uint32_t buf = used & 1, t = tmem + ((uint32_t)(quad * 32) << 16) + buf * kAcc + half;
+                if (q.nk > 0) {
+                    if (!wait<kPair>(&t_full[buf], (used >> 1) & 1u, abort_flag, a.wait_ns)) break;
+                    tc_fence_after();
+                    used++;
+                }
+                bool freed = q.nk == 0;
+                auto last_read = [&] {        // the accumulator is read: the next tile may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tmem_free(&t_empty[buf]);
+                    freed = true;
+                };
+                if (es == 2 && q.nk > 0) {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < n; c0 += kWide) {
+                        uint32_t v[kWide];
+#pragma unroll
+                        for (int h = 0; h < kWide; h += 32) tmem_ld32(t + c0 + h, *reinterpret_cast<uint32_t(*)[32]>(v + h));
+                        tmem_wait_ld();
+                        if (c0 + kWide >= n) last_read();
+                        put_16(c0, v);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c0 = 0; c0 < n; c0 += 32) {
+                        uint32_t u[32];
+                        float v[kBlock];
+                        if (q.nk > 0) {
+                            tmem_ld32(t + c0, u);
+                            tmem_wait_ld();
+                            if (c0 + 32 >= n) last_read();
+                        }
+#pragma unroll
+                        for (int i = 0; i < kBlock; i++) v[i] = q.nk > 0 && PLANES == 1 ? __uint_as_float(u[i]) : 0.0f;
+                        if (es == 4) {
+                            put_f32(c0, v);
+                        } else {              // an expert without rows: zeros
+                            for (int row = 0; row < live; row++)
+                                if (c0 + lane < n) static_cast<uint16_t *>(a.out)[at + row * pitch + c0 + lane] = 0;
                         }
                     }
                 }
-                used++;
-                continue;
-            }
-#pragma unroll (PLANES == 3 ? BN / 32 : 1)
-            for (int c0 = 0; c0 < BN; c0 += 32) {
-                if (q.n0 + c0 >= cols) break;
-                uint32_t v[32];
-                if (PLANES == 3) {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = __float_as_uint(acc[PLANES == 3 ? c0 + i : 0]);
-                } else if (q.nk > 0) {
-                    tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (used & 1) * kAcc + c0, v);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 32; i++) v[i] = 0u;
-                }
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 32; i += 4)
-                    *reinterpret_cast<uint4 *>(st + lane * kStageLd + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                __syncwarp();
-                auto bias_at = [&](int i) -> float { return MODE == kForward ? bias_s[c0 + i] : 0.0f; };
-                if (vec && es == 4) {
-                    const int cc = (lane & 7) * 4, col = q.n0 + c0 + cc;
-                    const float b0 = bias_at(cc), b1 = bias_at(cc + 1), b2 = bias_at(cc + 2), b3 = bias_at(cc + 3);
-                    float *o = static_cast<float *>(a.out) + at + col;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int row = i * 4 + (lane >> 3);
-                        float4 f = *reinterpret_cast<const float4 *>(st + row * kStageLd + cc);
-                        f.x += b0;
-                        f.y += b1;
-                        f.z += b2;
-                        f.w += b3;
-                        if (row < live && col < cols) *reinterpret_cast<float4 *>(o + row * pitch) = f;
-                    }
-                } else {
-                    const int col = q.n0 + c0 + lane;
-                    const float b = bias_at(lane);
-                    if (col < cols) {
-                        for (int row = 0; row < live; row++) {
-                            const float w = st[row * kStageLd + lane] + b;
-                            const int64_t o = at + row * pitch + col;
-                            if (a.out_dtype == FEQ_DTYPE_F32)
-                                static_cast<float *>(a.out)[o] = w;
-                            else if (a.out_dtype == FEQ_DTYPE_BF16)
-                                static_cast<__nv_bfloat16 *>(a.out)[o] = from_f32<__nv_bfloat16>(w);
-                            else
-                                static_cast<__half *>(a.out)[o] = from_f32<__half>(w);
-                        }
-                    }
-                }
-            }
-            if (PLANES == 1 && q.nk > 0) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tmem_free(&t_empty[used & 1]);
-                used++;
+                if (!freed) last_read();      // (none of its columns are in the matrix)
             }
         }
     }
@@ -806,6 +854,221 @@ bias_part_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const i
     }
 }
 
+// ---- few rows: the weights are read once, as they lie, and multiplied on the CUDA cores ----
+// A (row, component) pair is one line of an irrep's product; an expert's lines of an irrep are taken
+// four at a time, staged in shared memory as float4 (a contraction index, four lines), and two lines
+// share a multiply-add (f32x2).  The blocks of an expert without rows are not launched.
+constexpr int kLines = 4, kOutputs = 4, kFewWarps = 8, kFewDepth = 1024;
+
+struct Few {
+    const void *rows, *w, *b;                 // rows: x, or gy for gx
+    void *out;
+    const int32_t *offsets;
+    int64_t n, row, comp;                     // rows and their strides
+    int experts, cin, cout;
+};
+
+__device__ __forceinline__ uint64_t both(float v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ void fma2(uint64_t &d, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ void halves(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+
+// What a block works on: irrep rep of the blockIdx.y / reps-th expert that has rows (e < 0: there is none).
+struct Lines {
+    int e, rep, first, comps, count;
+    int64_t r0;
+};
+__device__ __forceinline__ Lines lines_of(const Few &a, const Comps &c, int32_t *off, int32_t *pre, int *found) {
+    if (threadIdx.x == 0) *found = -1;
+    lay_out(a.offsets, a.experts, a.n, off, pre, [](int32_t n) { return n > 0 ? 1 : 0; });
+    const int unit = blockIdx.y / c.reps, rep = blockIdx.y % c.reps;
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
+        if (pre[e] == unit && off[e + 1] > off[e]) *found = e;
+    __syncthreads();
+    const int e = *found;
+    if (e < 0) return {-1, 0, 0, 1, 0, 0};
+    const int comps = c.first[rep + 1] - c.first[rep];
+    return {e, rep, c.first[rep], comps, (int)min64((int64_t)(off[e + 1] - off[e]) * comps, INT32_MAX), off[e]};
+}
+
+// Rows that belong to no expert: zeros, by the first row of blocks.
+template <typename T>
+__device__ __forceinline__ void few_zeros(const Few &a, const Comps &c, const int32_t *off, int width) {
+    if (blockIdx.y != 0) return;
+    const int64_t lo = (int64_t)off[a.experts] * c.dim * width, hi = a.n * c.dim * width;
+    for (int64_t i = lo + (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < hi; i += (int64_t)gridDim.x * blockDim.x)
+        static_cast<T *>(a.out)[i] = from_f32<T>(0.0f);
+}
+
+// Stages the lines i0 .. i0 + 3 from contraction index k0 on (the last line again where there are fewer).
+// Index k lies at place_in<V>(k): lanes that read V indices each find the same one of theirs side by side.
+template <int V, int kDepth>
+__device__ __forceinline__ int place_in(int k) { return (k % V) * (kDepth / V) + k / V; }
+template <typename T, int V, int kDepth>
+__device__ __forceinline__ void stage_lines(const Few &a, const Lines &l, int i0, int k0, int depth, float4 *sh) {
+    __syncthreads();
+    const T *x[kLines];
+#pragma unroll
+    for (int i = 0; i < kLines; i++) {
+        const int line = min(i0 + i, l.count - 1);
+        x[i] = static_cast<const T *>(a.rows) + (l.r0 + line / l.comps) * a.row + (l.first + line % l.comps) * a.comp + k0;
+    }
+#pragma unroll 2
+    for (int k = threadIdx.x; k < depth; k += blockDim.x)
+        sh[place_in<V, kDepth>(k)] = make_float4(to_f32(x[0][k]), to_f32(x[1][k]), to_f32(x[2][k]), to_f32(x[3][k]));
+    __syncthreads();
+}
+
+// y: a warp has kOutputs output channels; its lanes share the input channels, V at a time and U steps
+// in flight together (about 32 bytes a lane and output).
+template <typename T, int V>
+__global__ void __launch_bounds__(kFewWarps * 32) few_rows_kernel(const __grid_constant__ Few a,
+                                                                  const __grid_constant__ Comps c) {
+    constexpr int U = V * sizeof(T) >= 16 ? 2 : V * sizeof(T) >= 8 ? 3 : V * sizeof(T) >= 4 ? 4 : 8;
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
+    __shared__ int found;
+    __shared__ float4 sh[kFewDepth];
+    const Lines l = lines_of(a, c, off, pre, &found);
+    few_zeros<T>(a, c, off, a.cout);
+    if (l.e < 0) return;
+    const int lane = threadIdx.x & 31, j0 = (blockIdx.x * kFewWarps + (threadIdx.x >> 5)) * kOutputs;
+    const int64_t matrix = (int64_t)l.e * c.reps + l.rep;
+    const T *w[kOutputs];
+#pragma unroll
+    for (int j = 0; j < kOutputs; j++)
+        w[j] = static_cast<const T *>(a.w) + (matrix * a.cout + min(j0 + j, a.cout - 1)) * a.cin;
+    for (int i0 = 0; i0 < l.count; i0 += kLines) {
+        uint64_t s[kOutputs][2];
+#pragma unroll
+        for (int j = 0; j < kOutputs; j++) s[j][0] = s[j][1] = 0;
+        for (int base = 0; base < a.cin; base += kFewDepth) {
+            const int depth = min(kFewDepth, a.cin - base);
+            stage_lines<T, V, kFewDepth>(a, l, i0, base, depth, sh);
+            for (int k0 = lane * V; k0 < depth; k0 += 32 * V * U) {
+                Pack<T, V> wv[U][kOutputs];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int k = k0 + u * 32 * V;
+#pragma unroll
+                    for (int j = 0; j < kOutputs; j++)
+                        if (k < depth) wv[u][j] = *reinterpret_cast<const Pack<T, V> *>(w[j] + base + k);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int k = k0 + u * 32 * V;
+                    if (k >= depth) break;
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(&sh[place_in<V, kFewDepth>(k + v)]);
+#pragma unroll
+                        for (int j = 0; j < kOutputs; j++) {
+                            const uint64_t g = both(to_f32(wv[u][j].v[v]));
+                            fma2(s[j][0], g, x.x);
+                            fma2(s[j][1], g, x.y);
+                        }
+                    }
+                }
+            }
+        }
+        // 16 sums over the lanes at once: each step halves the values and doubles the lanes they cover; lane t ends
+        // up with half of sum t % 16, the other half 16 lanes away
+        float t[kOutputs * kLines];
+#pragma unroll
+        for (int j = 0; j < kOutputs; j++) {
+            halves(s[j][0], t[j * kLines], t[j * kLines + 1]);
+            halves(s[j][1], t[j * kLines + 2], t[j * kLines + 3]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int i = 0; i < o; i++) {
+                const float keep = up ? t[i + o] : t[i], give = up ? t[i] : t[i + o];
+                t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+        t[0] += __shfl_xor_sync(0xffffffffu, t[0], 16);
+        const int j = j0 + lane / kLines, line = i0 + lane % kLines;
+        if (lane < 16 && j < a.cout && line < l.count) {
+            const int sc = a.b ? c.scalar_of[l.rep] : -1;
+            float y = t[0];
+            if (sc >= 0) y += to_f32(static_cast<const T *>(a.b)[((int64_t)l.e * c.scalars + sc) * a.cout + j]);
+            static_cast<T *>(a.out)[((l.r0 + line / l.comps) * c.dim + l.first + line % l.comps) * a.cout + j] = from_f32<T>(y);
+        }
+    }
+}
+
+// gx: a block has 32 V input channels (128 bytes of a row of the weights), lane by lane, so that there are
+// many blocks; its 16 warps share the output channels and are joined in their order.
+constexpr int kGxWarps = 16;
+template <typename T, int V>
+__global__ void __launch_bounds__(kGxWarps * 32) few_rows_gx_kernel(const __grid_constant__ Few a,
+                                                                    const __grid_constant__ Comps c) {
+    constexpr int U = 8;
+    __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
+    __shared__ int found;
+    __shared__ float4 sh[kFewDepth / 2];
+    __shared__ float part[kGxWarps][kLines][32 * V];
+    const Lines l = lines_of(a, c, off, pre, &found);
+    few_zeros<T>(a, c, off, a.cin);
+    if (l.e < 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = (blockIdx.x * 32 + lane) * V;
+    const T *w = static_cast<const T *>(a.w) + ((int64_t)l.e * c.reps + l.rep) * a.cin * a.cout + k;
+    for (int i0 = 0; i0 < l.count; i0 += kLines) {
+        uint64_t s[V][2];
+#pragma unroll
+        for (int v = 0; v < V; v++) s[v][0] = s[v][1] = 0;
+        for (int base = 0; base < a.cout; base += kFewDepth / 2) {
+            const int depth = min(kFewDepth / 2, a.cout - base);
+            stage_lines<T, 1, kFewDepth / 2>(a, l, i0, base, depth, sh);
+            for (int j0 = warp; k < a.cin && j0 < depth; j0 += kGxWarps * U) {
+                Pack<T, V> wv[U];
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (j0 + u * kGxWarps < depth)
+                        wv[u] = *reinterpret_cast<const Pack<T, V> *>(w + (int64_t)(base + j0 + u * kGxWarps) * a.cin);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const int j = j0 + u * kGxWarps;
+                    if (j >= depth) break;
+                    const ulonglong2 g = *reinterpret_cast<const ulonglong2 *>(&sh[j]);
+#pragma unroll
+                    for (int v = 0; v < V; v++) {
+                        const uint64_t f = both(to_f32(wv[u].v[v]));
+                        fma2(s[v][0], f, g.x);
+                        fma2(s[v][1], f, g.y);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            float t[kLines];
+            halves(s[v][0], t[0], t[1]);
+            halves(s[v][1], t[2], t[3]);
+#pragma unroll
+            for (int i = 0; i < kLines; i++) part[warp][i][v * 32 + lane] = t[i];
+        }
+        __syncthreads();
+        for (int t = threadIdx.x; t < kLines * 32 * V; t += kGxWarps * 32) {
+            const int i = t / (32 * V), col = t % (32 * V), line = i0 + i, at = blockIdx.x * 32 * V + col;
+            if (line < l.count && at < a.cin) {
+                float v = 0.0f;
+#pragma unroll
+                for (int h = 0; h < kGxWarps; h++) v += part[h][i][col % V * 32 + col / V];
+                static_cast<T *>(a.out)[((l.r0 + line / l.comps) * c.dim + l.first + line % l.comps) * a.cin + at] = from_f32<T>(v);
+            }
+        }
+    }
+}
+
 // Rows (rows, dim, n) with strides of their own -> planes (PLANES, rows, dim, npad) of 16-bit values,
 // zeros from n to npad (a multiple of 8).  PLANES 3: float32 as three bfloat16 summing to it.  With
 // `reps` > 0 the rows are weights, reps per expert, and experts without rows of their own are left out.
@@ -813,13 +1076,20 @@ template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
 pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, int64_t row, int64_t comp,
             uint16_t *__restrict__ dst, int reps, const int32_t *__restrict__ offsets) {
-    const int units = npad / 8;
+    const uint32_t units = npad / 8;
     const int64_t total = rows * dim * units, plane = rows * dim * (int64_t)npad;
+    const bool narrow = total < (int64_t)1 << 31;
     const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uint64_t)row * sizeof(T) | (uint64_t)comp * sizeof(T)) & 15) == 0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t rd = i / units;
+        int64_t rd, r;                        // (divisions of 32 bits where they do)
+        if (narrow) {
+            rd = (uint32_t)i / units;
+            r = (uint32_t)rd / (uint32_t)dim;
+        } else {
+            rd = i / units;
+            r = rd / dim;
+        }
         const int k0 = (int)(i - rd * units) * 8;
-        const int64_t r = dim == 1 ? rd : rd / dim;
         if (reps > 0 && offsets[r / reps + 1] <= offsets[r / reps]) continue;
         const T *s = src + r * row + (rd - r * dim) * comp + k0;
         T v[8];
@@ -829,6 +1099,20 @@ pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, i
                 *reinterpret_cast<Pack<T, 4> *>(v + 4) = *reinterpret_cast<const Pack<T, 4> *>(s + 4);
             } else {
                 *reinterpret_cast<Pack<T, 8> *>(v) = *reinterpret_cast<const Pack<T, 8> *>(s);
+            }
+        } else if (sizeof(T) == 2 && k0 + 10 <= n) {
+            // four words from the 4-byte boundary at or below the first element, a fifth where that is one behind
+            const uint32_t *w = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(s) & ~uintptr_t(3));
+            const bool behind = reinterpret_cast<uintptr_t>(s) & 2;
+            uint32_t d[5];
+#pragma unroll
+            for (int q = 0; q < 4; q++) d[q] = w[q];
+            d[4] = behind ? w[4] : 0u;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const uint32_t x = behind ? __funnelshift_r(d[q], d[q + 1], 16) : d[q];
+                reinterpret_cast<uint16_t *>(v)[2 * q] = (uint16_t)x;
+                reinterpret_cast<uint16_t *>(v)[2 * q + 1] = (uint16_t)(x >> 16);
             }
         } else {
 #pragma unroll
@@ -991,7 +1275,7 @@ static int tails_of(Operand *t, const Operand &o, const FeqExpertLinearArgs &q, 
 template <int MODE, int PLANES, int BN, bool kPair>
 static int launch(const CUtensorMap *m, Params a, const Comps &c, int64_t tiles, cudaStream_t s) {
     constexpr uint32_t stage = PLANES * (BM + (kPair ? BN / 2 : BN)) * 128;
-    constexpr uint32_t smem = 1024 + stages_of(stage) * stage + kStaging;
+    constexpr uint32_t staging = staging_bytes(PLANES, BN), smem = 1024 + stages_of(stage, staging) * stage + staging;
     auto kern = gemm_kernel<MODE, PLANES, BN, kPair>;
     FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (!kPair) {
@@ -1053,12 +1337,12 @@ static int run(const Operand &A, const Operand &B, const Operand *tails, Params 
 
 // Tiles of a row product: the widest whose tiles still fill the SMs (a wider tile reads its operands
 // fewer times); float32 keeps three planes of both operands in shared memory, which leaves room for
-// 128.  Pairs where 256-row tiles of the experts' average rows fill the SMs twice.
+// 128.  Pairs where 256-row tiles of the experts' average rows fill the pairs of SMs.
 static Tiling row_tiling(int planes, int64_t rows, int experts, int dim, int n) {
     Tiling t = {planes == 1 ? 256 : 128, false};
-    const int64_t units = (rows + BM - 1) / BM * dim;
+    const int64_t units = max64(rows / BM, min64(experts, rows)) * dim;      // row tiles, about
     while (t.bn > 64 && (n <= t.bn / 2 || units * ((n + t.bn - 1) / t.bn) < sm_count())) t.bn >>= 1;
-    t.pair = t.bn == 256 && rows / experts >= 2 * BM && rows / (2 * BM) * dim * ((n + 255) / 256) >= sm_count();
+    t.pair = t.bn == 256 && rows / experts >= 2 * BM && rows / (2 * BM) * dim * ((n + 255) / 256) >= sm_count() / 2;
     return t;
 }
 
@@ -1083,6 +1367,8 @@ int build_comps(const int32_t *lvals, int32_t n, Comps *c) {
         for (int m = 0; m < 2 * lvals[i] + 1; m++) c->rep[c->dim++] = (int8_t)i;
     }
     c->first[n] = (int16_t)c->dim;
+    for (int i = 0; i < n; i++) c->by_size[i] = (int8_t)i;
+    std::stable_sort(c->by_size, c->by_size + n, [&](int a, int b) { return lvals[a] > lvals[b]; });
     return FEQ_OK;
 }
 
@@ -1097,10 +1383,10 @@ int64_t grad_w_tiles(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
     return (int64_t)q.num_experts * c.reps * ((q.c_out + high - 1) / high) * ((q.c_in + t.bn - 1) / t.bn);
 }
 
-// Tiles of gW: pairs where they fill the SMs twice without being split.
+// Tiles of gW: pairs where they fill the pairs of SMs without being split.
 Tiling grad_w_tiling(const FeqExpertLinearArgs &q, const Comps &c) {
     Tiling t = {q.c_in <= 64 ? 64 : q.dtype == FEQ_DTYPE_F32 || q.c_in <= 128 ? 128 : 256, false};
-    if (t.bn == 256 && q.c_out > BM) t.pair = grad_w_tiles(q, c, {256, true}) >= 148;
+    if (t.bn == 256 && q.c_out > BM) t.pair = grad_w_tiles(q, c, {256, true}) >= 148 / 2;
     return t;
 }
 
@@ -1109,7 +1395,7 @@ Tiling grad_w_tiling(const FeqExpertLinearArgs &q, const Comps &c) {
 // than kLongestPart terms, so that the tensor cores' cut-off stays below 1e-4 of a 16-bit sum.
 int part_rows(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
     const int64_t base = grad_w_tiles(q, c, t);
-    const int64_t parts = t.pair ? 1 : (2 * 148 + base - 1) / base;
+    const int64_t ctas = t.pair ? 148 / 2 : 148, parts = base >= ctas ? 1 : (2 * ctas + base - 1) / base;
     int most = 1;
     for (int i = 0; i < c.reps; i++) most = std::max(most, c.first[i + 1] - c.first[i]);
     const int64_t longest = kLongestPart / most / 64 * 64;
@@ -1126,6 +1412,8 @@ using namespace feq::token;
 namespace feq {
 namespace elin {
 
+static bool few_rows(const FeqExpertLinearArgs &q, const Comps &c, bool grad_x);
+
 // Bytes of workspace that the call needs: the packed copies of operands that no tensor map
 // describes as they lie, and gW's partial sums.
 static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool backward) {
@@ -1134,10 +1422,11 @@ static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool 
         if (!mappable(p, q.dtype, rows, dim, n, row, comp)) ws.take(packed_bytes(q.dtype, rows, dim, n));
     };
     const int64_t matrices = (int64_t)q.num_experts * c.reps;
-    if (backward && (q.grad_x || q.grad_weight))
+    const bool products = backward ? q.grad_x && !few_rows(q, c, true) : !few_rows(q, c, false);
+    if (backward && (products || q.grad_weight))
         pack(q.grad_out, q.rows, c.dim, q.c_out, q.grad_row_stride, q.grad_comp_stride);
-    if (!backward || q.grad_x) pack(q.weight, matrices, q.c_out, q.c_in, (int64_t)q.c_out * q.c_in, q.c_in);
-    if (!backward || q.grad_weight) pack(q.x, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride);
+    if (products) pack(q.weight, matrices, q.c_out, q.c_in, (int64_t)q.c_out * q.c_in, q.c_in);
+    if (backward ? q.grad_weight != nullptr : products) pack(q.x, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride);
     if (backward && q.grad_weight) {
         const int planes = q.dtype == FEQ_DTYPE_F32 ? 3 : 1;
         ws.take(tail_bytes(planes, q.num_experts, c.dim, q.c_out));
@@ -1175,6 +1464,56 @@ static Params params(const FeqExpertLinearArgs &q) {
     a.status = q.status;
     a.wait_ns = wait_limit_ns();
     return a;
+}
+
+// Whether y or gx runs on the CUDA cores.  By the lines that an expert with rows has on average for an irrep
+// (both forms measured, y / gx in us, CUDA cores against tensor cores):
+//   float32: up to 16.  Three planes of the weights are written and read before the tensor cores start, 16
+//     bytes for each 4 (32 x 576 x 1000, 8 lines: 35/50 against 71/89; 16: 58/92 against 71/89).
+//   16-bit operands that have to be packed for the tensor cores: up to 8 (32 x 577 x 1001, 4 lines: 25/36
+//     against 42/44; 8: 38/64 against 42/44).
+//   16-bit operands read as they lie: up to 4 where the tiles of the experts with rows leave SMs without work
+//     (3 rows of 64 x 1024 x 2048: 11/22 against 16/21), else never (32 x 576 x 1000, 1 line: 23/19 against 17/21).
+static bool few_rows(const FeqExpertLinearArgs &q, const Comps &c, bool grad_x) {
+    const int64_t touched = min64(q.num_experts, q.rows) * c.reps, lines = q.rows * c.dim;
+    if (q.dtype == FEQ_DTYPE_F32) return lines <= 16 * touched;
+    const bool as_it_lies =
+        mappable(q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in, (int64_t)q.c_out * q.c_in, q.c_in) &&
+        (grad_x ? mappable(q.grad_out, q.dtype, q.rows, c.dim, q.c_out, q.grad_row_stride, q.grad_comp_stride)
+                : mappable(q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride));
+    if (!as_it_lies) return lines <= 8 * touched;
+    const int64_t tiles = touched * ((grad_x ? q.c_in : q.c_out) + 63) / 64;
+    return lines <= 4 * touched && tiles < sm_count();
+}
+
+template <int MODE>
+static int few_product(const FeqExpertLinearArgs &q, const Comps &c, cudaStream_t s) {
+    const bool fwd = MODE == kForward;
+    Few a = {};
+    a.rows = fwd ? q.x : q.grad_out;
+    a.row = fwd ? q.x_row_stride : q.grad_row_stride;
+    a.comp = fwd ? q.x_comp_stride : q.grad_comp_stride;
+    a.w = q.weight;
+    a.b = fwd ? q.bias : nullptr;
+    a.out = fwd ? q.out : q.grad_x;
+    a.offsets = q.offsets;
+    a.n = q.rows;
+    a.experts = q.num_experts;
+    a.cin = q.c_in;
+    a.cout = q.c_out;
+    const size_t es = dtype_bytes(q.dtype);
+    int vec = vector_elems((uint64_t)(uintptr_t)q.weight | (uint64_t)q.c_in * es, es);
+    if (!fwd && vec * es > 4) vec = (int)(4 / es);
+    FEQ_TOKEN_TYPE(q.dtype, FEQ_TOKEN_VEC(T, vec, {
+        constexpr int kPer = kFewWarps * kOutputs;
+        const unsigned gy = (unsigned)(min64(q.num_experts, q.rows) * c.reps);      // experts that can have rows
+        if (fwd)
+            few_rows_kernel<T, V><<<dim3((q.c_out + kPer - 1) / kPer, gy), kFewWarps * 32, 0, s>>>(a, c);
+        else if constexpr (V * sizeof(T) <= 4)
+            few_rows_gx_kernel<T, V><<<dim3((q.c_in + 32 * V - 1) / (32 * V), gy), kGxWarps * 32, 0, s>>>(a, c);
+    }))
+    FEQ_LAUNCH_CHECK();
+    return FEQ_OK;
 }
 
 static int join(const float *part, const FeqExpertLinearArgs &q, const Comps &c, int chunk_rows, int per, int64_t size,
@@ -1221,6 +1560,7 @@ extern "C" int feq_expert_linear_fwd(const FeqExpertLinearArgs *args, void *work
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if ((rc = elin::bind_context()) != FEQ_OK) return rc;
     ProfScope prof("expert_linear", s);
+    if (elin::few_rows(q, c, false)) return elin::few_product<elin::kForward>(q, c, s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
     elin::Operand x, w;
     rc = elin::operand(&x, q.x, q.dtype, q.rows, c.dim, q.c_in, q.x_row_stride, q.x_comp_stride, &ws, s);
@@ -1251,11 +1591,16 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
     ProfScope prof("expert_linear_bwd", s);
     WsCarver ws = {static_cast<char *>(workspace), 0, workspace_bytes};
     elin::Operand g, x, w;
-    if (q.grad_x || q.grad_weight) {
+    const bool few = q.grad_x && elin::few_rows(q, c, true);
+    if (few) {
+        rc = elin::few_product<elin::kGradX>(q, c, s);
+        if (rc != FEQ_OK) return rc;
+    }
+    if ((q.grad_x && !few) || q.grad_weight) {
         rc = elin::operand(&g, q.grad_out, q.dtype, q.rows, c.dim, q.c_out, q.grad_row_stride, q.grad_comp_stride, &ws, s);
         if (rc != FEQ_OK) return rc;
     }
-    if (q.grad_x) {
+    if (q.grad_x && !few) {
         rc = elin::operand(&w, q.weight, q.dtype, (int64_t)q.num_experts * c.reps, q.c_out, q.c_in,
                            (int64_t)q.c_out * q.c_in, q.c_in, &ws, s, c.reps, q.offsets);
         if (rc == FEQ_OK) rc = elin::row_product<elin::kGradX>(q, c, g, w, q.grad_x, s);
