@@ -15,7 +15,7 @@
 //               the next tile's products run
 // Large 16-bit products run on pairs of CTAs (cta_group::2, 256 x 256 tiles): each CTA loads its 128 rows
 // of A and half of B's, which takes a third off the traffic through shared memory (writes plus reads,
-// 24 -> 16 KB per 16 of K and 128 cycles, of the 128 B a cycle that it moves): MEASURE_PAIR
+// 24 -> 16 KB per 16 of K and 128 cycles, of the 128 B a cycle that it moves).
 // The contraction runs over channels in y and gx and over rows in gW; an operand whose channels
 // are not the contraction is read MN-major (the shared-memory tile as the copy leaves it), so
 // nothing is transposed; the last rows of an expert, where a chunk of 64 would reach into the next
