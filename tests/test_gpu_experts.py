@@ -16,7 +16,7 @@ import torch
 
 import flash_eq as fe
 from conftest import check_equivariance, rel_l2
-from flash_eq.cuda import token_ops
+from flash_eq.cuda import _lib, token_ops
 
 pytestmark = pytest.mark.gpu
 
@@ -417,6 +417,37 @@ def test_gradients_are_differentiable_once(cuda_device):
         g.sum().backward()
     assert torch.autograd.grad(fe.expert_dispatch(torch.randn(6, 3, device=cuda_device, requires_grad=True), r).sum(),
                                z, allow_unused=True) == (None,)
+
+
+@pytest.mark.parametrize("dtype,sizes,ci,co", [
+    (torch.bfloat16, [5000, 3000, 1, 4000], 512, 1024),     # tiles on pairs of CTAs
+    (torch.float16, [300, 77, 0, 500], 256, 320),           # tiles on one CTA
+    (torch.float32, [2000, 77, 0, 3000], 192, 256)], ids=["pairs", "single", "planes"])
+def test_expert_linear_short_wait_limit(cuda_device, dtype, sizes, ci, co):
+    """A wait past its limit ends the kernel with status 2, copies and products drained, and the next call is
+    right again.  (On single CTAs the waits are shorter than the polls before the first look at the timer.)"""
+    x, w, b, offsets, go = _linear_inputs(sizes, 3, (0,), ci, co, dtype, cuda_device)
+    want = _linear_reference(x, w, b, offsets, (0,), go)
+    lib = _lib.load()
+
+    def both(status):
+        y = token_ops.expert_linear_fwd(x, w, b, offsets, (0,), status=status)
+        return [y, *token_ops.expert_linear_bwd(go, x, w, offsets, (0,), status=status)]
+
+    for short in (True, False):
+        status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+        old = lib.feq_set_wait_limit_ns(1 if short else 0)
+        try:
+            got = both(status)
+            torch.cuda.synchronize()
+        finally:
+            lib.feq_set_wait_limit_ns(old)
+        if short and dtype != torch.float16:
+            assert int(status) == 2, "a 1 ns wait limit should have timed out at least one wait"
+        assert int(status) in ((0, 2) if short else (0,))
+        if int(status) == 0:
+            for g, r in zip(got, want):
+                assert rel_l2(g, r) < TOL[dtype]
 
 
 def test_expert_linear_empty(cuda_device):
