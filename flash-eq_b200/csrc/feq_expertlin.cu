@@ -49,7 +49,7 @@ constexpr int kThreads = (2 + kEpilogueWarps) * 32;
 constexpr uint32_t kBox = 64 * 128;                 // bytes of a 64-row, 64-channel box
 constexpr int kMaxStages = 8;
 constexpr int kSegment = 4;                         // chunks a float32 accumulator runs over
-constexpr int kLongestPart = 65536;                 // terms of one 16-bit sum over rows
+constexpr int kLongestF16 = 1 << 16, kLongestBf16 = 1 << 18;   // terms of one sum over rows
 // Staging of an epilogue warp: 32 rows of kBlock floats (float32 tiles, whose operand ring leaves less
 // room, 16 = 64 B of a row; else 32 = 128 B), padded by 16 bytes, and the bias of its columns.
 __host__ __device__ constexpr int block_floats(int planes) { return planes == 3 ? 16 : 32; }
@@ -929,9 +929,9 @@ __device__ __forceinline__ void stage_lines(const Few &a, const Lines &l, int i0
 // y: a warp has kOutputs output channels; its lanes share the input channels, V at a time and U steps
 // in flight together (about 32 bytes a lane and output).
 template <typename T, int V>
-__global__ void __launch_bounds__(kFewWarps * 32) few_rows_kernel(const __grid_constant__ Few a,
+__global__ void __launch_bounds__(kFewWarps * 32, V == 1 ? 3 : 1) few_rows_kernel(const __grid_constant__ Few a,
                                                                   const __grid_constant__ Comps c) {
-    constexpr int U = V * sizeof(T) >= 16 ? 2 : V * sizeof(T) >= 8 ? 3 : V * sizeof(T) >= 4 ? 4 : 8;
+    constexpr int U = V * sizeof(T) >= 16 ? 2 : V * sizeof(T) >= 8 ? 3 : 4;
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     __shared__ int found;
     __shared__ float4 sh[kFewDepth];
@@ -1391,14 +1391,15 @@ Tiling grad_w_tiling(const FeqExpertLinearArgs &q, const Comps &c) {
 }
 
 // Rows of one part of gW's contraction (0: an expert's rows are one part): the whole expert where its
-// tiles fill the SMs anyway, else enough parts for about two tiles a SM, of 256 rows at least; never more
-// than kLongestPart terms, so that the tensor cores' cut-off stays below 1e-4 of a 16-bit sum.
+// tiles fill the SMs anyway, else enough parts for about two tiles a SM, of 256 rows at least.  A 16-bit
+// sum is never longer than kLongest terms, which keeps the tensor cores' cut-off (1.2e-9 of the sum a term) below
+// half of what rounding the result costs: 8e-5 against 2.1e-4 in float16, 3e-4 against 1.7e-3 in bfloat16.
 int part_rows(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
     const int64_t base = grad_w_tiles(q, c, t);
     const int64_t ctas = t.pair ? 148 / 2 : 148, parts = base >= ctas ? 1 : (2 * ctas + base - 1) / base;
     int most = 1;
     for (int i = 0; i < c.reps; i++) most = std::max(most, c.first[i + 1] - c.first[i]);
-    const int64_t longest = kLongestPart / most / 64 * 64;
+    const int64_t longest = (q.dtype == FEQ_DTYPE_F16 ? kLongestF16 : kLongestBf16) / most / 64 * 64;
     if (parts <= 1) return q.dtype != FEQ_DTYPE_F32 && q.rows > longest ? (int)longest : 0;
     return (int)min64(longest, max64(256, (q.rows / q.num_experts / parts + 63) / 64 * 64));
 }

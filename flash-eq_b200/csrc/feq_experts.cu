@@ -50,19 +50,22 @@ __device__ __forceinline__ uint32_t rank_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One warp chooses the experts of one token, L logits a lane; lane j < top_k ends up with choice j
-// (id -1: none).
+// A token's logits, L a lane (-inf past the last expert).
 template <typename T, int L>
-__device__ __forceinline__ void choose(const Route &a, int64_t n, int &my_id, float &my_w) {
-    const int lane = threadIdx.x & 31;
-    const T *row = static_cast<const T *>(a.logits) + n * a.stride;
-    float v[L];
-    uint32_t key[L], top = 0;
+__device__ __forceinline__ void logits_of(const T *row, int experts, float (&v)[L]) {
 #pragma unroll
     for (int i = 0; i < L; i++) {
-        const int e = i * 32 + lane;
-        v[i] = e < a.experts ? to_f32(row[e]) : -INFINITY;
+        const int e = i * 32 + (threadIdx.x & 31);
+        v[i] = e < experts ? to_f32(row[e]) : -INFINITY;
     }
+}
+
+// One warp chooses the experts of one token from its logits; lane j < top_k ends up with choice j
+// (id -1: none).
+template <int L>
+__device__ __forceinline__ void choose(const Route &a, const float (&v)[L], int &my_id, float &my_w) {
+    const int lane = threadIdx.x & 31;
+    uint32_t key[L], top = 0;
 #pragma unroll
     for (int i = 0; i < L; i++) {
         key[i] = rank_key(v[i]);
@@ -185,10 +188,16 @@ __global__ void __launch_bounds__(kSmallThreads) route_small_kernel(const Route 
     int32_t *hist = sh, *count = hist + warps * nk, *starts = count + nk;
     int16_t *key = reinterpret_cast<int16_t *>(starts + nk);
     for (int i = threadIdx.x; i < warps * nk; i += blockDim.x) hist[i] = 0;
+    const T *logits = static_cast<const T *>(a.logits);
+    float v[L], next[L];
+    if (warp < (int)a.tokens) logits_of<T, L>(logits + warp * a.stride, a.experts, next);
     for (int n = warp; n < (int)a.tokens; n += warps) {
         int id;
         float w;
-        choose<T, L>(a, n, id, w);
+#pragma unroll
+        for (int i = 0; i < L; i++) v[i] = next[i];
+        if (n + warps < (int)a.tokens) logits_of<T, L>(logits + (n + warps) * a.stride, a.experts, next);
+        choose<L>(a, v, id, w);
         if (lane < a.top_k) {
             const int p = n * a.top_k + lane;
             a.ids[p] = id;
@@ -222,10 +231,16 @@ __global__ void __launch_bounds__(kPlaceThreads) route_choose_kernel(const Route
     for (int i = threadIdx.x; i < nk; i += blockDim.x) sh[i] = 0;
     __syncthreads();
     const int64_t n0 = (int64_t)blockIdx.x * a.tokens_per_block, n1 = min64(n0 + a.tokens_per_block, a.tokens);
+    const T *logits = static_cast<const T *>(a.logits);
+    float v[L], next[L];                      // the next token's logits are on their way while one chooses
+    if (n0 + warp < n1) logits_of<T, L>(logits + (n0 + warp) * a.stride, a.experts, next);
     for (int64_t n = n0 + warp; n < n1; n += warps) {
         int id;
         float w;
-        choose<T, L>(a, n, id, w);
+#pragma unroll
+        for (int i = 0; i < L; i++) v[i] = next[i];
+        if (n + warps < n1) logits_of<T, L>(logits + (n + warps) * a.stride, a.experts, next);
+        choose<L>(a, v, id, w);
         if (lane < a.top_k) {
             const int64_t p = n * a.top_k + lane;
             a.ids[p] = id;
@@ -295,8 +310,10 @@ __global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(const Route 
     warp_place(key, lo, hi, hist + warp * nk, a.slots + p0);
 }
 
-// grad_logits of the weights; one warp per token.
-template <typename T>
+// grad_logits of the weights; one warp per token.  With share = sum_j w_j g_j a chosen expert has
+// w_j (g_j - share), another one 0 (normalize) or -p_e share, where p_e = exp(l_e - l_first) w_first: the first
+// choice's weight is 1 / the sum of the softmax over all.
+template <typename T, int L>
 __global__ void __launch_bounds__(256)
 route_bwd_kernel(const T *__restrict__ logits, int64_t stride, int64_t tokens, int E, int k, int normalize,
                  const int32_t *__restrict__ ids, const float *__restrict__ w, const float *__restrict__ gw,
@@ -304,35 +321,27 @@ route_bwd_kernel(const T *__restrict__ logits, int64_t stride, int64_t tokens, i
     const int lane = threadIdx.x & 31;
     const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (n >= tokens) return;
-    const int id = lane < k ? ids[n * k + lane] : -1;
+    float v[L] = {};                          // read before the choice that it is compared with is known
+    if (!normalize) logits_of<T, L>(logits + n * stride, E, v);
+    int id = lane < k ? ids[n * k + lane] : -1;
+    if (id >= E) id = -1;
     const float wj = id >= 0 ? w[n * k + lane] : 0.0f, g = id >= 0 ? gw[n * k + lane] : 0.0f;
-    const float share = lane_sum(wj * g, 32);
-    float biggest = 0.0f, total = 1.0f;
-    if (!normalize) {
-        const int first = __shfl_sync(0xffffffffu, id, 0);
-        if (first >= 0 && first < E) {
-            biggest = to_f32(logits[n * stride + first]);
-            float s = 0.0f;
-            for (int e = lane; e < E; e += 32) s += expf(to_f32(logits[n * stride + e]) - biggest);
-            total = lane_sum(s, 32);
-        }
+    const float share = lane_sum(wj * g, 32), first_w = __shfl_sync(0xffffffffu, wj, 0);
+    const int first = __shfl_sync(0xffffffffu, id, 0);
+    const bool all = !normalize && first >= 0;
+    float biggest = 0.0f;
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        const float u = __shfl_sync(0xffffffffu, v[i], max(first, 0) & 31);
+        if (all && first >> 5 == i) biggest = u;
     }
-    for (int e0 = 0; e0 < E; e0 += 32) {
-        const int e = e0 + lane;
-        float v = 0.0f, spread = 0.0f;
-        for (int j = 0; j < k; j++) {
-            const int ej = __shfl_sync(0xffffffffu, id, j);
-            const float a = __shfl_sync(0xffffffffu, wj, j), b = __shfl_sync(0xffffffffu, g, j);
-            if (ej == e) {
-                v = a * b;
-                spread = a;
-            }
-        }
-        if (e < E) {
-            if (!normalize) spread = expf(to_f32(logits[n * stride + e]) - biggest) / total;
-            out[n * E + e] = from_f32<T>(v - spread * share);
-        }
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        const int e = i * 32 + lane;
+        if (e < E) out[n * E + e] = from_f32<T>(all ? -expf(v[i] - biggest) * first_w * share : 0.0f);
     }
+    __syncwarp();
+    if (id >= 0) out[n * E + id] = from_f32<T>(wj * (g - share));
 }
 
 // ---- rows ------------------------------------------------------------------------------------
@@ -502,10 +511,11 @@ __global__ void __launch_bounds__(kRowThreads) combine_bwd_kernel(const Rows a) 
     }
 }
 
-// Blocks of choosing and placing: of 256 pairs (8 warps choose a few tokens each, one after the other)
-// up to a million pairs, then larger, which keeps the table of counts small.
+// Blocks of choosing and placing: about 2048 of them, of 64 pairs at least (the 8 warps of a block choose
+// its tokens one after the other: 20 000 x 2 of 16 experts in blocks of 256 pairs took 20 us, of which a
+// warp waited 16 times for a row).
 int route_plan(int64_t tokens, int top_k, int *per) {
-    const int64_t pairs = min64(kPlacePairs, max64(256, tokens * top_k / 4096));
+    const int64_t pairs = min64(kPlacePairs, max64(64, tokens * top_k / 2048));
     const int t = (int)max64(1, pairs / top_k);
     *per = t;
     return (int)((tokens + t - 1) / t);
@@ -610,9 +620,11 @@ extern "C" int feq_expert_route_bwd(const void *logits, int64_t tokens, int64_t 
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     ProfScope prof("expert_route_bwd", s);
     const unsigned grid = (unsigned)((tokens + 7) / 8);
-    FEQ_TOKEN_TYPE(dtype, experts::route_bwd_kernel<T><<<grid, 256, 0, s>>>(
-                              static_cast<const T *>(logits), stride, tokens, num_experts, top_k, normalize, ids,
-                              weights, grad_weights, static_cast<T *>(grad_logits));)
+    FEQ_TOKEN_TYPE(dtype, FEQ_EXPERTS_PER_LANE(num_experts, {
+        experts::route_bwd_kernel<T, L><<<grid, 256, 0, s>>>(static_cast<const T *>(logits), stride, tokens, num_experts,
+                                                             top_k, normalize, ids, weights, grad_weights,
+                                                             static_cast<T *>(grad_logits));
+    }))
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
