@@ -16,6 +16,8 @@
 // Products that enter the row's sums, and u mean(g w u), are rounded before they are added: in rows of
 // two the terms of gx cancel down to eps / v of their size, and a product kept longer on one side only
 // would be what is left.
+// Measured: 1 M x 128 float32 forward 170 us (6.0 TB/s), backward 272 us (5.6 TB/s); 16384 x 2048 bfloat16 36 and
+// 55 us, there bound by instructions (60 % of the issue slots); 20011 x 1001 float16 forward 29 us.
 // Rows wider than kMaxWidth go through kernels that stream the row from L2 instead.
 #include <algorithm>
 
@@ -482,8 +484,8 @@ __global__ void __launch_bounds__(kBlock) wide_columns_kernel(const Args a) {
 // How a row is spread: vectors of `vec` elements, `elems` elements a thread, `tpr` threads a row.
 // Vectors are 16 bytes where every row of every tensor starts equally far behind a 16-byte boundary
 // (then `shift` unless that is 0), else as wide as the addresses allow.  16 elements a thread, so that
-// the sums across threads are a small part of the work, but 8 in short rows, where 16 would leave
-// fewer than 4 threads side by side on a row.
+// the sums across threads are a small part of the work (1 M x 128 float32 backward: 272 us, with 8 elements
+// 312), but 8 in short rows, where 16 would leave fewer than 4 threads side by side on a row.
 struct Spread {
     int vec, elems, tpr, threads;
     bool shift;
