@@ -1339,8 +1339,7 @@ static int run(const Operand &A, const Operand &B, const Operand *tails, Params 
 }
 
 // Tiles of a row product: the widest whose tiles still fill the SMs (a wider tile reads its operands
-// fewer times: 64 rows of 64 experts, 1024 x 2048 bfloat16, 57 us at 256 columns and 100 at 64; but 3 rows of
-// them, 48 tiles of 64 columns, 16 us and 19 at 256); float32 keeps three planes of both operands in shared
+// fewer times: 64 rows of 64 experts, 1024 x 2048 bfloat16, 57 us at 256 columns and 100 at 64); float32 keeps three planes of both operands in shared
 // memory, which leaves room for 128.  Pairs where 256-row tiles of the experts' average rows fill the pairs
 // of SMs (65536 x 1024 -> 2048: y 230 us against 242 on single CTAs, gx 222 against 249, gW 239 against 254).
 static Tiling row_tiling(int planes, int64_t rows, int experts, int dim, int n) {
