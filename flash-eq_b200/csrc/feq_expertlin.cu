@@ -5,8 +5,8 @@
 //   gW[e, i]    = sum over rows r of e and components p of irrep i of gy[r, p] x[r, p]^T
 //   gb[e, s]    = sum over rows r of e of gy[r, component of scalar s]
 //
-// Rows of expert e are offsets[e] .. offsets[e + 1); rows from offsets[experts] on belong to none and
-// give zeros.  The offsets stay on the device: every kernel lays out its own work from them.
+// Rows of expert e are offsets[e] .. offsets[e + 1), offsets[0] counting as 0; rows from offsets[experts] on
+// belong to none and give zeros.  The offsets stay on the device: every kernel lays out its own work from them.
 //
 // The three products are one persistent tcgen05 kernel (gemm_kernel), a CTA per SM, 128 x BN tiles:
 //   warp 0      loads: tensor-map copies of 64-deep operand chunks into a ring (no multicast)
@@ -1093,7 +1093,7 @@ pack_kernel(const T *__restrict__ src, int64_t rows, int dim, int n, int npad, i
             r = rd / dim;
         }
         const int k0 = (int)(i - rd * units) * 8;
-        if (reps > 0 && offsets[r / reps + 1] <= offsets[r / reps]) continue;
+        if (reps > 0 && offsets[r / reps + 1] <= (r < reps ? 0 : offsets[r / reps])) continue;
         const T *s = src + r * row + (rd - r * dim) * comp + k0;
         T v[8];
         if (wide && k0 + 8 <= n) {

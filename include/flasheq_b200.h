@@ -598,7 +598,8 @@ int feq_expert_combine_bwd(const void *grad_out, int64_t grad_stride, const void
 /* The experts' linear maps on rows sorted by expert: x (rows, dim, c_in) with dim = sum(2 l + 1)
  * over lvals (lvals = {0}: plain rows), weight (num_experts, n_lvals, c_out, c_in), bias
  * (num_experts, scalars, c_out) on the l = 0 components or NULL; out (rows, dim, c_out)
- * contiguous.  Rows of expert e are offsets[e] .. offsets[e + 1) (device, int32); rows from
+ * contiguous.  Rows of expert e are offsets[e] .. offsets[e + 1) (device, int32; offsets[0] counts
+ * as 0, the others are taken as never decreasing and at most rows); rows from
  * offsets[num_experts] on give zeros.  All tensors have the type `dtype`.
  * The backward fills those of grad_x (rows, dim, c_in), grad_weight and grad_bias that are not
  * NULL.  status (may be NULL): 2 when a tensor-core wait timed out (result invalid).
