@@ -756,30 +756,42 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
 }
 
 // The rows of each expert that do not fill a chunk of 64, padded with rows of zeros: (planes, experts * 64,
-// dim, np) from (planes, rows, dim, n) 16-bit values, np a multiple of 8.  One block a row of the result.
+// dim, np) from (planes, rows, dim, n) 16-bit values, np a multiple of 8.  A block has kTailRows rows of the
+// result; blockIdx.y: the operand.
+constexpr int kTailRows = 8;
+struct Tail {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t row, comp, plane;
+    int n, np;
+};
+struct Tails {
+    Tail t[2];
+    int planes, dim;
+};
 __global__ void __launch_bounds__(256)
-tails_kernel(const uint16_t *__restrict__ src, int64_t row, int64_t comp, int64_t plane, int planes, int dim, int n, int np,
-             const int32_t *__restrict__ offsets, int experts, int64_t rows, uint16_t *__restrict__ dst) {
-    const int e = blockIdx.x / BK, i = blockIdx.x % BK;
+tails_kernel(const __grid_constant__ Tails a, const int32_t *__restrict__ offsets, int experts, int64_t rows) {
+    const Tail &t = a.t[blockIdx.y];
+    const int e = blockIdx.x / (BK / kTailRows), i0 = blockIdx.x % (BK / kTailRows) * kTailRows;
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     lay_out(offsets, experts, rows, off, pre, [](int32_t) { return 0; });
     const int live = (off[e + 1] - off[e]) % BK;
     if (live == 0) return;                    // this expert has no such chunk: nothing reads it
-    const int64_t r = off[e + 1] - live + i;
-    const bool wide = ((reinterpret_cast<uintptr_t>(src) | (uint64_t)(row | comp | plane) * 2) & 15) == 0;
-    const int units = np / 8;
-    for (int u = threadIdx.x; u < planes * dim * units; u += 256) {
-        const int pl = u / (dim * units), d = u / units % dim, k0 = u % units * 8;
-        const uint16_t *s = src + pl * plane + r * row + d * comp + k0;
+    const bool wide = ((reinterpret_cast<uintptr_t>(t.src) | (uint64_t)(t.row | t.comp | t.plane) * 2) & 15) == 0;
+    const int units = t.np / 8, line = a.dim * units;
+    for (int u = threadIdx.x; u < a.planes * kTailRows * line; u += 256) {
+        const int pl = u / (kTailRows * line), i = i0 + u / line % kTailRows, d = u / units % a.dim, k0 = u % units * 8;
+        const int64_t r = off[e + 1] - live + i;
+        const uint16_t *s = t.src + pl * t.plane + r * t.row + d * t.comp + k0;
         Pack<uint16_t, 8> o;
-        if (i < live && wide && k0 + 8 <= n) {
+        if (i < live && wide && k0 + 8 <= t.n) {
             o = *reinterpret_cast<const Pack<uint16_t, 8> *>(s);
         } else {
 #pragma unroll
-            for (int q = 0; q < 8; q++) o.v[q] = i < live && k0 + q < n ? s[q] : (uint16_t)0;
+            for (int q = 0; q < 8; q++) o.v[q] = i < live && k0 + q < t.n ? s[q] : (uint16_t)0;
         }
         *reinterpret_cast<Pack<uint16_t, 8> *>(
-            dst + (((int64_t)pl * experts * BK + blockIdx.x) * dim + d) * np + k0) = o;
+            t.dst + ((((int64_t)pl * experts + e) * BK + i) * a.dim + d) * t.np + k0) = o;
     }
 }
 
@@ -812,13 +824,14 @@ join_kernel(const float *__restrict__ part, const int32_t *offsets, int experts,
 // gb, step 1: the columns of one part of an expert's rows (kBiasRows of them) and one scalar.  A warp
 // reads V channels a lane of every 8th row; the warps' sums are joined in their order.
 constexpr int kBiasRows = 256;
-template <typename T, int V>
+// kWhole: no expert has more rows than a part, and its sum is written at once (out).
+template <typename T, int V, bool kWhole>
 __global__ void __launch_bounds__(256)
 bias_part_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const int32_t *offsets, int experts, int64_t rows,
-                 int cout, const __grid_constant__ Comps c, float *__restrict__ part) {
+                 int cout, const __grid_constant__ Comps c, float *__restrict__ part, T *__restrict__ out) {
     __shared__ int32_t off[kMaxExperts + 1], pre[kMaxExperts + 1];
     __shared__ float sh[8][32 * V + 1];
-    lay_out(offsets, experts, rows, off, pre, [](int32_t n) { return (n + kBiasRows - 1) / kBiasRows; });
+    lay_out(offsets, experts, rows, off, pre, [](int32_t n) { return kWhole ? 1 : (n + kBiasRows - 1) / kBiasRows; });
     const int unit = blockIdx.x / c.scalars, sc = blockIdx.x % c.scalars;
     if (unit >= pre[experts]) return;
     int lo = 0, hi = experts;                 // the expert of this unit: pre[lo] <= unit < pre[lo + 1]
@@ -853,7 +866,9 @@ bias_part_kernel(const T *__restrict__ g, int64_t g_row, int64_t g_comp, const i
         float v = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; k++) v += sh[k][i];
-        part[((int64_t)unit * c.scalars + sc) * cout + col] = v;
+        const int64_t at = ((int64_t)unit * c.scalars + sc) * cout + col;
+        if (kWhole) out[at] = from_f32<T>(v);
+        else part[at] = v;
     }
 }
 
@@ -1258,19 +1273,26 @@ static int operand(Operand *o, const void *p, int dtype, int64_t rows, int dim, 
 
 static size_t tail_bytes(int planes, int experts, int dim, int n) { return (size_t)planes * experts * BK * dim * pad8(n) * 2; }
 
-// The padded last rows of an operand's experts.
-static int tails_of(Operand *t, const Operand &o, const FeqExpertLinearArgs &q, WsCarver *ws, cudaStream_t s) {
-    const int np = pad8(o.n);
-    *t = o;
-    t->rows = (int64_t)q.num_experts * BK;
-    t->comp = np;
-    t->row = (int64_t)o.dim * np;
-    t->plane = t->rows * t->row;
-    t->base = ws->take(tail_bytes(o.planes, q.num_experts, o.dim, o.n));
-    if (ws->used > ws->cap) return FEQ_ERR_WORKSPACE;
-    tails_kernel<<<(unsigned)t->rows, 256, 0, s>>>(static_cast<const uint16_t *>(o.base), o.row, o.comp, o.plane, o.planes,
-                                                   o.dim, o.n, np, q.offsets, q.num_experts, q.rows,
-                                                   static_cast<uint16_t *>(const_cast<void *>(t->base)));
+// The padded last rows of both operands' experts.
+static int tails_of(Operand (&t)[2], const Operand &A, const Operand &B, const FeqExpertLinearArgs &q, WsCarver *ws,
+                    cudaStream_t s) {
+    Tails a = {};
+    a.planes = A.planes;
+    a.dim = A.dim;
+    for (int i = 0; i < 2; i++) {
+        const Operand &o = i ? B : A;
+        const int np = pad8(o.n);
+        t[i] = o;
+        t[i].rows = (int64_t)q.num_experts * BK;
+        t[i].comp = np;
+        t[i].row = (int64_t)o.dim * np;
+        t[i].plane = t[i].rows * t[i].row;
+        void *dst = ws->take(tail_bytes(o.planes, q.num_experts, o.dim, o.n));
+        if (ws->used > ws->cap) return FEQ_ERR_WORKSPACE;
+        t[i].base = dst;
+        a.t[i] = {static_cast<const uint16_t *>(o.base), static_cast<uint16_t *>(dst), o.row, o.comp, o.plane, o.n, np};
+    }
+    tails_kernel<<<dim3((unsigned)t[0].rows / kTailRows, 2), 256, 0, s>>>(a, q.offsets, q.num_experts, q.rows);
     FEQ_LAUNCH_CHECK();
     return FEQ_OK;
 }
@@ -1406,7 +1428,8 @@ int part_rows(const FeqExpertLinearArgs &q, const Comps &c, Tiling t) {
     for (int i = 0; i < c.reps; i++) most = std::max(most, c.first[i + 1] - c.first[i]);
     const int64_t longest = (q.dtype == FEQ_DTYPE_F16 ? kLongestF16 : kLongestBf16) / most / 64 * 64;
     if (parts <= 1) return q.dtype != FEQ_DTYPE_F32 && q.rows > longest ? (int)longest : 0;
-    return (int)min64(longest, max64(256, (q.rows / q.num_experts / parts + 63) / 64 * 64));
+    const int64_t part = min64(longest, max64(256, (q.rows / q.num_experts / parts + 63) / 64 * 64));
+    return q.rows <= part ? 0 : (int)part;    // (no expert has more rows than one part)
 }
 
 }  // namespace elin
@@ -1440,7 +1463,7 @@ static size_t workspace_need(const FeqExpertLinearArgs &q, const Comps &c, bool 
         const int part = part_rows(q, c, grad_w_tiling(q, c));
         if (part > 0) ws.take((size_t)(q.rows / part + q.num_experts) * c.reps * q.c_in * q.c_out * sizeof(float));
     }
-    if (backward && q.grad_bias && c.scalars)
+    if (backward && q.grad_bias && c.scalars && q.rows > kBiasRows)
         ws.take((size_t)(q.rows / kBiasRows + min64(q.num_experts, q.rows)) * c.scalars * q.c_out * sizeof(float));
     return (ws.used + 255) & ~size_t(255);       // in any order of the regions
 }
@@ -1632,8 +1655,7 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
         a.idesc = elin::instr(q.dtype, t, true, true);
         const int64_t tiles = parts * (elin::grad_w_tiles(q, c, t) / q.num_experts);
         elin::Operand tails[2];
-        rc = elin::tails_of(&tails[0], g, q, &ws, s);
-        if (rc == FEQ_OK) rc = elin::tails_of(&tails[1], x, q, &ws, s);
+        rc = elin::tails_of(tails, g, x, q, &ws, s);
         if (rc == FEQ_OK) rc = elin::run<elin::kGradW>(g, x, tails, a, c, t, tiles, s);
         if (rc != FEQ_OK) return rc;
         if (a.split) {
@@ -1643,21 +1665,26 @@ extern "C" int feq_expert_linear_bwd(const FeqExpertLinearArgs *args, void *work
         }
     }
     if (q.grad_bias && c.scalars) {
-        const int64_t units = q.rows / elin::kBiasRows + min64(q.num_experts, q.rows);
-        float *part = static_cast<float *>(ws.take((size_t)units * c.scalars * q.c_out * sizeof(float)));
-        if (ws.used > ws.cap) return FEQ_ERR_WORKSPACE;
+        const bool whole = q.rows <= elin::kBiasRows;
+        const int64_t units = whole ? q.num_experts : q.rows / elin::kBiasRows + min64(q.num_experts, q.rows);
+        float *part = nullptr;
+        if (!whole) {
+            part = static_cast<float *>(ws.take((size_t)units * c.scalars * q.c_out * sizeof(float)));
+            if (ws.used > ws.cap) return FEQ_ERR_WORKSPACE;
+        }
         const int vec = vector_elems((uint64_t)(uintptr_t)q.grad_out | (uint64_t)q.grad_row_stride * es |
                                          (uint64_t)q.grad_comp_stride * es | (uint64_t)q.c_out * es, es);
-        const unsigned gx = (unsigned)(units * c.scalars);
         FEQ_TOKEN_TYPE(q.dtype, FEQ_TOKEN_VEC(T, vec, {
-            const dim3 grid(gx, (unsigned)((q.c_out + 32 * V - 1) / (32 * V)));
-            elin::bias_part_kernel<T, V><<<grid, 256, 0, s>>>(static_cast<const T *>(q.grad_out), q.grad_row_stride,
-                                                              q.grad_comp_stride, q.offsets, q.num_experts, q.rows,
-                                                              q.c_out, c, part);
+            const dim3 grid((unsigned)(units * c.scalars), (unsigned)((q.c_out + 32 * V - 1) / (32 * V)));
+            auto kern = whole ? elin::bias_part_kernel<T, V, true> : elin::bias_part_kernel<T, V, false>;
+            kern<<<grid, 256, 0, s>>>(static_cast<const T *>(q.grad_out), q.grad_row_stride, q.grad_comp_stride, q.offsets,
+                                      q.num_experts, q.rows, q.c_out, c, part, static_cast<T *>(q.grad_bias));
         }))
         FEQ_LAUNCH_CHECK();
-        rc = elin::join(part, q, c, elin::kBiasRows, c.scalars, q.c_out, q.grad_bias, s);
-        if (rc != FEQ_OK) return rc;
+        if (!whole) {
+            rc = elin::join(part, q, c, elin::kBiasRows, c.scalars, q.c_out, q.grad_bias, s);
+            if (rc != FEQ_OK) return rc;
+        }
     }
     return FEQ_OK;
 }
