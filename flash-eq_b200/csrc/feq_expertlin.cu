@@ -758,7 +758,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CU
 // The rows of each expert that do not fill a chunk of 64, padded with rows of zeros: (planes, experts * 64,
 // dim, np) from (planes, rows, dim, n) 16-bit values, np a multiple of 8.  A block has kTailRows rows of the
 // result; blockIdx.y: the operand.
-constexpr int kTailRows = 8;
+constexpr int kTailRows = 4;
 struct Tail {
     const uint16_t *src;
     uint16_t *dst;
@@ -779,6 +779,7 @@ tails_kernel(const __grid_constant__ Tails a, const int32_t *__restrict__ offset
     if (live == 0) return;                    // this expert has no such chunk: nothing reads it
     const bool wide = ((reinterpret_cast<uintptr_t>(t.src) | (uint64_t)(t.row | t.comp | t.plane) * 2) & 15) == 0;
     const int units = t.np / 8, line = a.dim * units;
+#pragma unroll 4
     for (int u = threadIdx.x; u < a.planes * kTailRows * line; u += 256) {
         const int pl = u / (kTailRows * line), i = i0 + u / line % kTailRows, d = u / units % a.dim, k0 = u % units * 8;
         const int64_t r = off[e + 1] - live + i;

@@ -10,7 +10,7 @@
 // the centred sum of squares are exact two-pass sums over registers and the row is read once.
 // A thread owns the same columns for every row of its group, so w and b are read once per
 // thread and, backwards, gw and gb are summed in registers over the group's rows; the groups of
-// a block join in shared memory and the blocks in a second kernel, all in a fixed order.  The next
+// a block join in shared memory and the blocks in a second kernel, in float64 and a fixed order.  The next
 // rows are copied to shared memory while the current one is summed.  Rows of odd widths are read in 16-byte vectors that
 // straddle their ends (row_shift).
 // Products that enter the row's sums, and u mean(g w u), are rounded before they are added: in rows of
@@ -336,10 +336,22 @@ __global__ void __launch_bounds__(B, B == kBlock ? 3 : 1) forward_kernel(const A
     }
 }
 
+// Slices of the groups in the join of a block: so many that every thread has a column of one.
+__host__ __device__ __forceinline__ int join_slices(int width, int threads, int groups) {
+    const int n = threads / (2 * width);
+    return n < 1 ? 1 : n < groups ? n : groups;
+}
+// Shared memory of the join.
+inline size_t join_bytes(int width, int threads, int groups) {
+    const size_t sums = ((size_t)groups * 2 * width * sizeof(float) + 7) & ~size_t(7);
+    const int slices = join_slices(width, threads, groups);
+    return sums + (slices > 1 ? (size_t)slices * 2 * width * sizeof(double) : 0);
+}
+
 template <typename T, int V, int E, bool kShift, int B>
 __global__ void __launch_bounds__(B, B == kBlock ? 2 : 1) backward_kernel(const Args a) {
     __shared__ __align__(16) float red[2][2][16];
-    extern __shared__ __align__(16) uint8_t ring[];      // the rings of x and g; at the end (2, width) sums
+    extern __shared__ __align__(16) uint8_t ring[];      // the rings of x and g; at the end the join
     int slot = 0;
     const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), group = threadIdx.x / tpr, groups = blockDim.x / tpr;
     const int64_t first = (int64_t)blockIdx.x * groups + group, every = (int64_t)gridDim.x * groups;
@@ -403,47 +415,59 @@ __global__ void __launch_bounds__(B, B == kBlock ? 2 : 1) backward_kernel(const 
         r += every;
     }
     if (!a.partial) return;
-    // join the groups in their order
+    // Join the groups: their sums side by side (gw and gb of every column, group after group), then slices of the
+    // groups by different threads, then the slices; in float64, in a fixed order.
     float *sums = reinterpret_cast<float *>(ring);
+    const int cols = 2 * a.width, slices = join_slices(a.width, blockDim.x, groups), per = (groups + slices - 1) / slices;
+    double *sliced = reinterpret_cast<double *>(ring + (((size_t)groups * cols * sizeof(float) + 7) & ~size_t(7)));
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
-    for (int k = 0; k < groups; k++) {
-        if (group == k) {
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int c = x.c0 + e / V * x.pitch + e % V;
-                if (c >= 0 && c < a.width) {
-                    sums[c] = (k ? sums[c] : 0.0f) + gw[e];
-                    sums[a.width + c] = (k ? sums[a.width + c] : 0.0f) + gb[e];
-                }
-            }
+    for (int e = 0; e < E; e++) {
+        const int c = x.c0 + e / V * x.pitch + e % V;
+        if (c >= 0 && c < a.width) {
+            sums[group * cols + c] = gw[e];
+            sums[group * cols + a.width + c] = gb[e];
         }
-        __syncthreads();
     }
-    float *out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
-    for (int i = threadIdx.x; i < 2 * a.width; i += blockDim.x) out[i] = sums[i];
+    __syncthreads();
+    float *out = a.partial + (int64_t)blockIdx.x * cols;
+    for (int i = threadIdx.x; i < cols * slices; i += blockDim.x) {
+        const int col = i % cols, k0 = i / cols * per, k1 = min(k0 + per, groups);
+        double v = 0.0;
+        for (int k = k0; k < k1; k++) v += sums[k * cols + col];
+        if (slices == 1) out[col] = (float)v;
+        else sliced[i] = v;
+    }
+    if (slices == 1) return;
+    __syncthreads();
+    for (int col = threadIdx.x; col < cols; col += blockDim.x) {
+        double v = 0.0;
+        for (int k = 0; k < slices; k++) v += sliced[k * cols + col];
+        out[col] = (float)v;
+    }
 }
 
 // gw, gb = the sum of the blocks' partial sums: 32 columns a block, 32 warps over the partials,
-// joined in warp order.
+// joined in warp order, in float64.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 reduce_kernel(const float *__restrict__ partial, int blocks, int width, int param_f32, void *gw, void *gb) {
-    __shared__ float sh[32][kReduceCols + 1];
+    __shared__ double sh[32][kReduceCols + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int i = blockIdx.x * kReduceCols + lane;        // of 2 * width
-    float s = 0.0f;
+    double s = 0.0;
     if (i < 2 * width)
         for (int k = warp; k < blocks; k += 32) s += partial[(int64_t)k * 2 * width + i];
     sh[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && i < 2 * width) {
-        float v = 0.0f;
+        double v = 0.0;
         for (int k = 0; k < 32; k++) v += sh[k][lane];
         if (i < width) {
-            if (gw) param_put<T>(gw, param_f32, i, v);
+            if (gw) param_put<T>(gw, param_f32, i, (float)v);
         } else if (gb) {
-            param_put<T>(gb, param_f32, i - width, v);
+            param_put<T>(gb, param_f32, i - width, (float)v);
         }
     }
 }
@@ -703,7 +727,8 @@ extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, con
         const lnorm::Spread sp = lnorm::spread(at, width, es);
         a.tpr = sp.tpr;
         blocks = (int)lnorm::backward_blocks(rows, width, sp.threads / sp.tpr);
-        const size_t smem = std::max(2 * lnorm::ring_bytes(sp, es), params ? (size_t)width * 2 * sizeof(float) : 0);
+        const size_t smem = std::max(2 * lnorm::ring_bytes(sp, es),
+                                     params ? lnorm::join_bytes(width, sp.threads, sp.threads / sp.tpr) : 0);
         auto go = [&](auto kern) -> int {
             if (smem > 48 * 1024 - 1024)
                 FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
