@@ -415,6 +415,19 @@ __global__ void __launch_bounds__(B, B == kBlock ? 2 : 1) backward_kernel(const 
         r += every;
     }
     if (!a.partial) return;
+    if (groups == 1) {                        // a row takes the block: nothing to join
+        float *out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int c = x.c0 + e / V * x.pitch + e % V;
+            if (c >= 0 && c < a.width) {
+                out[c] = gw[e];
+                out[a.width + c] = gb[e];
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        return;
+    }
     // Join the groups: their sums side by side (gw and gb of every column, group after group), then slices of the
     // groups by different threads, then the slices; in float64, in a fixed order.
     float *sums = reinterpret_cast<float *>(ring);
@@ -728,7 +741,7 @@ extern "C" int feq_layer_norm_bwd(const void *grad_out, int64_t grad_stride, con
         a.tpr = sp.tpr;
         blocks = (int)lnorm::backward_blocks(rows, width, sp.threads / sp.tpr);
         const size_t smem = std::max(2 * lnorm::ring_bytes(sp, es),
-                                     params ? lnorm::join_bytes(width, sp.threads, sp.threads / sp.tpr) : 0);
+                                     params && sp.tpr < sp.threads ? lnorm::join_bytes(width, sp.threads, sp.threads / sp.tpr) : 0);
         auto go = [&](auto kern) -> int {
             if (smem > 48 * 1024 - 1024)
                 FEQ_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
