@@ -16,9 +16,9 @@
 // Large 16-bit products run on pairs of CTAs (cta_group::2, 256 x 256 tiles): each CTA loads its 128 rows
 // of A and half of B's, which takes a third off the traffic through shared memory (writes plus reads,
 // 24 -> 16 KB per 16 of K and 128 cycles, of the 128 B a cycle that it moves).  Measured at 65536 rows, 32
-// experts, 1024 -> 2048 bfloat16: y 235 us, gx 224, gW 240 (1.17 to 1.22 PFLOP/s at the 1.33 GHz of the power cap,
-// the tensor pipe 70 % busy); float32, 16384 rows, 8 experts, 576 -> 1152: 107 us (1.21 PFLOP/s executed) + 26 of
-// packing; 40000 x 9 rows, 64 -> 128 float32: 74 / 66 / 92 us + 149 of packing, bound by HBM.
+// experts, 1024 -> 2048 bfloat16: y 225 us, gx 218, gW 235 (1.17 to 1.26 PFLOP/s at the 1.33 GHz of the power cap,
+// the tensor pipe 70 % busy); float32, 16384 rows, 8 experts, 576 -> 1152: 105 us (1.24 PFLOP/s executed) + 25 of
+// packing; 40000 x 9 rows, 64 -> 128 float32: 72 / 66 / 91 us + 150 of packing, bound by HBM.
 // The contraction runs over channels in y and gx and over rows in gW; an operand whose channels
 // are not the contraction is read MN-major (the shared-memory tile as the copy leaves it), so
 // nothing is transposed; the last rows of an expert, where a chunk of 64 would reach into the next

@@ -16,8 +16,8 @@
 // Products that enter the row's sums, and u mean(g w u), are rounded before they are added: in rows of
 // two the terms of gx cancel down to eps / v of their size, and a product kept longer on one side only
 // would be what is left.
-// Measured: 1 M x 128 float32 forward 170 us (6.0 TB/s), backward 272 us (5.6 TB/s); 16384 x 2048 bfloat16 36 and
-// 55 us, there bound by instructions (60 % of the issue slots); 20011 x 1001 float16 forward 29 us.
+// Measured: 1 M x 128 float32 forward 170 us (6.0 TB/s), backward 272 to 283 us (5.4 to 5.7 TB/s); 16384 x 2048 bfloat16 32 and
+// 55 us, the backward bound by instructions (60 % of the issue slots); 20011 x 1001 float16 forward 27 us.
 // Rows wider than kMaxWidth go through kernels that stream the row from L2 instead.
 #include <algorithm>
 #include <type_traits>
